@@ -42,6 +42,11 @@ cudaError_t uq_merge_wait_dispatch(const void*, int, size_t, unsigned int, size_
 cudaError_t uq_merge_dispatch(const float*, const float*, int, size_t, int, void*, cudaStream_t);
 cudaError_t uq_layout_dispatch(int, uint8_t*, uint8_t*, uint8_t*, uint8_t*, uint8_t*, long long, int, int, int, int, int, cudaStream_t);
 cudaError_t uq_merge_packed_dispatch(const float*, int, size_t, int, void*, cudaStream_t);
+cudaError_t uq_plan_dispatch(const int32_t*, const int32_t*, int, int32_t*, long long, const int32_t*, long long, int64_t*, int32_t*, int, long long, int, int, int sms, cudaStream_t);
+cudaError_t uq_rms_norm_dispatch(const void*, const void*, const void*, void*, uint8_t*, uint8_t*, long long, int, int, float, int sms, cudaStream_t);
+cudaError_t uq_silu_mul_dispatch(const void*, uint8_t*, uint8_t*, long long, int, int, cudaStream_t);
+size_t uq_fp4_linear_scratch(long long, int);
+cudaError_t uq_fp4_linear_dispatch(const void*, const uint8_t*, const uint8_t*, const uint8_t*, void*, void*, long long, int, int, int, unsigned int* status, cudaStream_t, int* launches);
 
 namespace {
 
@@ -295,6 +300,39 @@ int uqb_cache_from_upstream_launch(const uint8_t* slots_in, uint8_t* kc, uint8_t
                                    int slot_bytes, void* stream) {
   cudaError_t e = uq_layout_dispatch(1, kc, ks, vc, vs, const_cast<uint8_t*>(slots_in), pages, HKV, PAGE, D, slot_bytes, 0, reinterpret_cast<cudaStream_t>(stream));
   if (e == cudaSuccess && pages > 0) g_launches += 1;
+  return (int)e;
+}
+
+// ---- the operators around a layer's attention --------------------------------------------------------------------
+int uqb_plan_step_launch(const int32_t* seq_lens, const int32_t* starts, int K, int32_t* block_table, long long row_stride, const int32_t* free_pages, long long n_free,
+                         int64_t* slots, int32_t* taken, int B, long long T, int PAGE, int max_pages, void* stream) {
+  cudaError_t e = uq_plan_dispatch(seq_lens, starts, K, block_table, row_stride, free_pages, n_free, slots, taken, B, T, PAGE, max_pages, sm_count(),
+                                   reinterpret_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) g_launches += 1;
+  return (int)e;
+}
+
+int uqb_rms_norm_mx8_launch(const void* x, const void* residual, const void* weight, void* sum, uint8_t* codes, uint8_t* scales, long long rows, int H, int dtype,
+                            float eps, void* stream) {
+  cudaError_t e = uq_rms_norm_dispatch(x, residual, weight, sum, codes, scales, rows, H, dtype, eps, sm_count(), reinterpret_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess && rows > 0) g_launches += 1;
+  return (int)e;
+}
+
+int uqb_silu_mul_mx8_launch(const void* x, uint8_t* codes, uint8_t* scales, long long rows, int F, int dtype, void* stream) {
+  cudaError_t e = uq_silu_mul_dispatch(x, codes, scales, rows, F, dtype, reinterpret_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess && rows > 0) g_launches += 1;
+  return (int)e;
+}
+
+size_t uqb_fp4_linear_scratch_bytes(long long M, int K) { return uq_fp4_linear_scratch(M, K); }
+
+int uqb_fp4_linear_launch(const void* x, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, void* out, void* scratch, long long M, int N, int K, int out_dtype,
+                          void* stream) {
+  unsigned int* status = status_ptr();
+  int launches = 0;
+  cudaError_t e = uq_fp4_linear_dispatch(x, xs, wc, ws, out, scratch, M, N, K, out_dtype, status, reinterpret_cast<cudaStream_t>(stream), &launches);
+  g_launches += (unsigned)launches;
   return (int)e;
 }
 

@@ -68,6 +68,13 @@ def _slots_for(workspace, B, K, HQ, HKV, D, n_pages, device):
     return min(want, workspace.numel() // one) if one else want
 
 
+def plan_step(seq_lens, query_start_loc, block_table, page_size, num_tokens, *, free_pages=None, slots=None):
+    """The step's slot map (slot_mapping of append_kv), and with free_pages the block table's new pages, from the requests'
+    lengths on the GPU (uq_cuda.plan_step): safe inside a captured step, nothing is read on the host.  query_start_loc int32
+    [B+1] as eligible() takes it, or K for a uniform step.  Returns (slots int64 [num_tokens], taken int32 [1] or None)."""
+    return uq_cuda.plan_step(seq_lens, query_start_loc, block_table, page_size, num_tokens, free_pages=free_pages, slots=slots)
+
+
 def append_kv(kc, ks, vc, vs, key, value, slot_mapping, *, rotate_k=False, rule="ceil", c=None, kernel=None):
     """Quantize new key/value [T, Hkv, D] and write them at flat slots (slot = physical_page * PAGE + offset), the
     cache-append hook of an engine (reference uqmt/vllm_adapter.py:48-59); one kernel launch, a decode step's tokens or a

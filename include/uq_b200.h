@@ -81,6 +81,49 @@ int uqb_append_nvfp4_ex_launch(uint8_t* kc, uint8_t* ks, uint8_t* vc, uint8_t* v
  * out may be x: the reference's fwht (uqmt/quant.py:84-98, rotate_kq :105-107) for the queries. */
 int uqb_fwht_launch(const void* x, void* out, long long rows, int D, int dtype, void* stream);
 
+/* ---- the operators around a layer's attention (no counterpart in the reference) ------------------------------------ */
+
+/* Block tables and slot maps of a step from its requests' lengths, in one launch.
+ *   seq_lens    int32 [B], B <= 16384: tokens stored per request once this step's are in (what the verify launch takes);
+ *   new tokens  K > 0: K per request (starts NULL); K == 0 with starts int32 [B + 1]: those between a request's start and the
+ *               next (the engine's query_start_loc); K == 0 and starts NULL: all of them (whole prompts, packed in order).
+ *               They are the last tokens of their request, in the rows starts[b].. of the step's token axis;
+ *   block_table int32 [B, max_pages], rows row_stride elements apart: a request holds the pages of the tokens it had before;
+ *               the pages it needs on top are written behind them, nothing else of the table is;
+ *   free_pages  int32 [n_free], with taken: the needed pages come from here, in the order of the requests; taken (int32 [1])
+ *               gets their number.  It may exceed n_free: the entries that could not be filled are -1 then, and so are the
+ *               slots of their tokens.  taken NULL (n_free 0): the table is complete already and is only read;
+ *   slots       int64 [T]: the slot (page * PAGE + offset) of every new token, as the append launches take it; -1 for rows
+ *               behind the last request's tokens (a padded step), for tokens before position 0 (more new tokens than stored
+ *               ones) and for positions beyond the table. */
+int uqb_plan_step_launch(const int32_t* seq_lens, const int32_t* starts, int K, int32_t* block_table, long long row_stride, const int32_t* free_pages,
+                         long long n_free, int64_t* slots, int32_t* taken, int B, long long T, int PAGE, int max_pages, void* stream);
+
+/* 8-bit rows: e4m3 codes [rows, H] and one scale byte per 32 channels [rows, H/32], value = code * 2^(byte - 127), byte the
+ * least with which nothing is clipped (0 for a group of zeros).  Values that are not finite get the NaN code.
+ * dtype 0 = fp32, 1 = bf16, 2 = fp16 (of x, residual, weight and sum); H (F) a multiple of 32; codes 8-byte aligned, the
+ * others 16.
+ *   rms_norm:  s = x + residual (NULL: x), codes of s / sqrt(mean(s^2) + eps) * weight (NULL: ones), in fp32 throughout; sum
+ *              [rows, H] gets s rounded to dtype (NULL exactly when residual is; may be x or residual itself).  H <= 32768, eps > 0.
+ *   silu_mul:  x [rows, 2 F] = gates, then factors: codes of g / (1 + exp(-g)) * u. */
+int uqb_rms_norm_mx8_launch(const void* x, const void* residual, const void* weight, void* sum, uint8_t* codes, uint8_t* scales, long long rows, int H,
+                            int dtype, float eps, void* stream);
+int uqb_silu_mul_mx8_launch(const void* x, uint8_t* codes, uint8_t* scales, long long rows, int F, int dtype, void* stream);
+
+/* Products with a 4-bit weight: out[m, n] = sum_k x[m, k] * w[n, k], M rows (a decode or verify step's tokens), fp32 sums.
+ *   wc, ws      the weight as one stream of the paged cache with PAGE = 128, D = 128: codes [ceil(N/128), ceil(K/128), 128, 64],
+ *               scales [ceil(N/128), ceil(K/128), 128, 4]; row n of the weight is token n % 128 of page n / 128, channels
+ *               128 h.. are head h.  uqb_append_ex_launch writes it (key = the weight as [N, K/128, 128], slots 0..N-1);
+ *               channels behind K and rows behind N have finite scales (the append leaves zero codes there when they are zero).
+ *   x, xs       xs NULL: x is bf16 [M, K], taken as two e4m3 planes (exact but for what lies under 2^-21 of a group's largest),
+ *               scratch holds uqb_fp4_linear_scratch_bytes(M, K) bytes; else x e4m3 [M, K], xs its scale bytes [M, K/32].
+ *   out         [M, N], out_dtype 0 = fp32, 1 = bf16, 2 = fp16.
+ * K a multiple of 32, wc 32-byte aligned, x / ws / out / scratch 16, xs 4.  A row of x that holds NaN or infinity (bf16), or a
+ * NaN code, gives NaN in its outputs; other rows are not touched by it. */
+size_t uqb_fp4_linear_scratch_bytes(long long M, int K);
+int uqb_fp4_linear_launch(const void* x, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, void* out, void* scratch, long long M, int N, int K,
+                          int out_dtype, void* stream);
+
 /* ---- the upstream engines' slot layout ------------------------------------------------------------ */
 
 /* Byte permute between this library's four cache arrays and the upstream engines' single array of per-token slots

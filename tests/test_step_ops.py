@@ -1,0 +1,496 @@
+"""The operators around a layer's attention - plan_step, rms_norm_mx8, silu_mul_mx8, fp4_linear - against plain implementations in
+64 bits (numpy), their refusals, and a layer's step made of them.
+
+Tolerances.  A rounding to e4m3 is off by at most half a step: 2^-4 of the value, or 2^-10 of the scale below 2^-6 of it.  The
+value that is rounded carries an fp32 error: sums of at most 32768 squares as a tree of 8 + log2 stages, a reciprocal root (2 ulp),
+three products, an exponential (2 ulp) - under 32 roundings of 2^-24, taken as YERR = 2^-19 of the value.  So a code has to be
+one that some y within (1 +- YERR) of the 64-bit value rounds to, and a scale one that some such maximum asks for."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from all_quant_b200 import uq_cuda, vllm_adapter
+
+YERR = 2.0 ** -19
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+FP4 = np.array([0, .5, 1, 1.5, 2, 3, 4, 6, -0., -.5, -1, -1.5, -2, -3, -4, -6])
+
+
+# ---------------------------------------------------------------------------------------------------- plain forms, 64 bits
+def e4m3(v):
+    """Nearest e4m3 value, ties to even."""
+    v = np.asarray(v, np.float64)
+    e = np.maximum(np.frexp(v)[1] - 1, -6)
+    step = np.ldexp(1.0, e - 3)
+    return np.clip(np.rint(v / step) * step, -448, 448)
+
+
+def exponent(amax):
+    """The least E with amax <= 448 * 2^E, -127 for zero."""
+    m, e = np.frexp(np.asarray(amax, np.float64))
+    return np.where(amax > 0, np.maximum(e - 9 + (m > 0.875), -127), -127)
+
+
+def check_mx8(codes, scales, y):
+    """codes e4m3 tensor [..., n], scales uint8 [..., n/32] against the 64-bit rows y."""
+    y = np.asarray(y, np.float64)
+    got = codes.float().cpu().numpy().astype(np.float64).reshape(-1, 32)
+    E = scales.cpu().numpy().astype(np.int64).reshape(-1) - 127
+    g = y.reshape(-1, 32)
+    amax = np.abs(g).max(1)
+    assert (E >= exponent(amax * (1 - YERR))).all() and (E <= exponent(amax * (1 + YERR))).all()
+    scaled = np.ldexp(g, -E[:, None])
+    a, b = e4m3(scaled * (1 - YERR)), e4m3(scaled * (1 + YERR))
+    assert ((got >= np.minimum(a, b)) & (got <= np.maximum(a, b))).all()
+    assert (np.abs(np.ldexp(got, E[:, None]) - g) <= (2.0 ** -4 + YERR) * np.abs(g) + np.ldexp(2.0 ** -10, E)[:, None]).all()
+
+
+def weight64(wc, ws, n, K):
+    c, s = wc.cpu().numpy(), ws.cpu().numpy().astype(np.int64)
+    tiles, ks = c.shape[:2]
+    w = np.stack([FP4[c & 15], FP4[c >> 4]], -1).reshape(tiles, ks, 128, 4, 32)
+    w = np.ldexp(w, (s - 127)[..., None])
+    return w.transpose(0, 2, 1, 3, 4).reshape(tiles * 128, ks * 128)[:n, :K]
+
+
+def mx8_values(codes, scales):
+    c = codes.float().cpu().numpy().astype(np.float64)
+    s = scales.cpu().numpy().astype(np.int64) - 127
+    return np.ldexp(c.reshape(s.shape + (32,)), s[..., None]).reshape(c.shape)
+
+
+def check_linear(got, x64, w64, dtype, split=False):
+    """fp32 sums of exact products, in any order of blocks of 32: every partial sum is at most A = sum |x w|, every one of the
+    K / 32 + 32 additions on the way to an output off by at most 2^-22 of that; then one rounding to the output's type.  Rows
+    split from bf16: what lies under 2^-21 of a group's largest value is lost."""
+    y, A = x64 @ w64.T, np.abs(x64) @ np.abs(w64).T
+    K = x64.shape[1]
+    tol = (K / 32 + 32) * 2.0 ** -22 * A + torch.finfo(dtype).eps / 2 * np.abs(y) + torch.finfo(dtype).tiny
+    if split:
+        top = np.abs(x64).reshape(-1, K // 32, 32).max(2).repeat(32, 1)
+        tol = tol + 2.0 ** -21 * top @ np.abs(w64).T
+    assert (np.abs(got.double().cpu().numpy() - y) <= tol).all()
+
+
+def plan64(lens, new, table, page, T, free=None, starts=None):
+    """One request and one token at a time."""
+    table, slots, taken = table.copy(), np.full(T, -1, np.int64), 0
+    first = 0
+    for b, (n, k) in enumerate(zip(lens, new)):
+        n = max(n, 0)
+        k = max(k, 0)
+        mp = table.shape[1]
+        held = min(-(-max(n - k, 0) // page), mp)
+        if free is not None:
+            for j in range(held, min(-(-n // page), mp)):
+                table[b, j] = free[taken] if taken < len(free) else -1
+                taken += 1
+        at = first if starts is None else starts[b]
+        for i in range(k):
+            p = n - k + i
+            if 0 <= p and at + i < T and p // page < mp and table[b, p // page] >= 0:
+                slots[at + i] = int(table[b, p // page]) * page + p % page
+        first += k
+    return table, slots, taken
+
+
+# ------------------------------------------------------------------------------------------------------- refusals (CPU)
+FAKE = 0x7F0000000000
+
+
+def _p(i, delta=0):
+    return ctypes.c_void_p(FAKE + i * 0x1000000 + delta)
+
+
+@pytest.mark.parametrize("over", [dict(B=-1), dict(B=16385), dict(K=-1), dict(T=-1), dict(T=1 << 31), dict(PAGE=0), dict(max_pages=-1), dict(stride=7),
+                                  dict(n_free=-1), dict(lens=None), dict(table=None), dict(slots=None), dict(n_free=4, taken=None), dict(n_free=4, free=None),
+                                  dict(B=16384, max_pages=1 << 18, stride=1 << 18), dict(K=2, starts=_p(1))])
+def test_plan_refuses(over):
+    a = dict(lens=_p(0), starts=None, K=1, table=_p(2), stride=8, free=_p(3), n_free=0, slots=_p(4), taken=_p(5), B=4, T=4, PAGE=16, max_pages=8)
+    a.update(over)
+    L = uq_cuda.lib()
+    n0 = L.uqb_launch_count()
+    assert L.uqb_plan_step_launch(*[a[k] for k in ("lens", "starts", "K", "table", "stride", "free", "n_free", "slots", "taken", "B", "T", "PAGE", "max_pages")], None) == 1
+    assert L.uqb_launch_count() == n0
+
+
+@pytest.mark.parametrize("over", [dict(H=0), dict(H=48), dict(H=32800), dict(rows=-1), dict(dtype=3), dict(eps=0.0), dict(eps=float("nan")), dict(sum=None), dict(r=None),
+                                  dict(x=None), dict(x=_p(0, 8)), dict(w=_p(2, 2)), dict(codes=_p(4, 4)), dict(scales=None), dict(sum=_p(3, 8))])
+def test_norm_refuses(over):
+    a = dict(x=_p(0), r=_p(1), w=_p(2), sum=_p(3), codes=_p(4), scales=_p(5), rows=4, H=64, dtype=1, eps=1e-6)
+    a.update(over)
+    L = uq_cuda.lib()
+    n0 = L.uqb_launch_count()
+    assert L.uqb_rms_norm_mx8_launch(*[a[k] for k in ("x", "r", "w", "sum", "codes", "scales", "rows", "H", "dtype", "eps")], None) == 1
+    assert L.uqb_launch_count() == n0
+
+
+@pytest.mark.parametrize("over", [dict(F=0), dict(F=40), dict(F=(1 << 20) + 32), dict(rows=-1), dict(dtype=-1), dict(x=None), dict(x=_p(0, 2)), dict(codes=_p(1, 4)), dict(scales=None)])
+def test_silu_refuses(over):
+    a = dict(x=_p(0), codes=_p(1), scales=_p(2), rows=4, F=64, dtype=1)
+    a.update(over)
+    L = uq_cuda.lib()
+    n0 = L.uqb_launch_count()
+    assert L.uqb_silu_mul_mx8_launch(*[a[k] for k in ("x", "codes", "scales", "rows", "F", "dtype")], None) == 1
+    assert L.uqb_launch_count() == n0
+
+
+@pytest.mark.parametrize("over", [dict(M=-1), dict(M=(1 << 24) + 1), dict(N=0), dict(K=0), dict(K=48), dict(dtype=3), dict(x=None), dict(wc=None), dict(ws=None), dict(out=None),
+                                  dict(x=_p(0, 8)), dict(wc=_p(2, 16)), dict(ws=_p(3, 8)), dict(out=_p(4, 8)), dict(xs=_p(1, 2)), dict(xs=None, scratch=None),
+                                  dict(xs=None, scratch=_p(5, 8))])
+def test_linear_refuses(over):
+    a = dict(x=_p(0), xs=_p(1), wc=_p(2), ws=_p(3), out=_p(4), scratch=_p(5), M=4, N=128, K=64, dtype=1)
+    a.update(over)
+    L = uq_cuda.lib()
+    n0 = L.uqb_launch_count()
+    assert L.uqb_fp4_linear_launch(*[a[k] for k in ("x", "xs", "wc", "ws", "out", "scratch", "M", "N", "K", "dtype")], None) == 1
+    assert L.uqb_launch_count() == n0
+
+
+def test_scratch_sizes_agree():
+    for M, K in ((1, 32), (8, 4096), (64, 8192), (65, 96), (1000, 32768)):
+        assert uq_cuda.fp4_linear_scratch_bytes(M, K) == uq_cuda._fp4_scratch(M, K)
+    assert uq_cuda.fp4_linear_scratch_bytes(0, 64) == 0 and uq_cuda.fp4_linear_scratch_bytes(4, 40) == 0
+
+
+def test_cpu_tensors_are_refused():
+    z = torch.zeros
+    for call in (lambda: uq_cuda.plan_step(z(2, dtype=torch.int32), 1, z(2, 4, dtype=torch.int32), 16, 2), lambda: uq_cuda.rms_norm_mx8(z(2, 64)),
+                 lambda: uq_cuda.silu_mul_mx8(z(2, 64)), lambda: uq_cuda.pack_fp4_weight(z(2, 64)),
+                 lambda: uq_cuda.fp4_linear(z(1, 128, dtype=torch.bfloat16), z(1, 1, 128, 64, dtype=torch.uint8), z(1, 1, 128, 4, dtype=torch.uint8))):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+# ---------------------------------------------------------------------------------------------------------------- plan
+gpu = pytest.mark.gpu
+
+
+def _plan_case(rng, B, page, lo, hi, new_lo, new_hi, spare=0, extra_cols=0):
+    lens = rng.integers(lo, hi + 1, B)
+    new = lens.copy() if new_hi < 0 else np.minimum(rng.integers(new_lo, new_hi + 1, B), lens)
+    held, total = -(-(lens - new) // page), -(-lens // page)
+    perm = rng.permutation(int(total.sum()) + spare).astype(np.int32)
+    table = np.full((B, max(int(total.max(initial=0)), 1) + extra_cols), -7, np.int32)
+    at = 0
+    for b in range(B):
+        table[b, :held[b]] = perm[at:at + held[b]]
+        at += held[b]
+    return lens, new, table, perm[at:]
+
+
+def _run_plan(lens, new, table, page, T, free, mode):
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    bt = dev(table)
+    arg = {"starts": dev(starts), "uniform": int(new[0]) if len(new) else 1, "whole": None}[mode]
+    slots, taken = uq_cuda.plan_step(dev(lens.astype(np.int32)), arg, bt, page, T, free_pages=None if free is None else dev(free))
+    return bt.cpu().numpy(), slots.cpu().numpy(), None if taken is None else int(taken)
+
+
+@gpu
+@pytest.mark.parametrize("B,page,lo,hi,new_lo,new_hi,mode", [
+    (1, 64, 1, 1, 1, 1, "uniform"), (2, 64, 777, 1000, 4, 4, "uniform"), (5, 16, 1, 40, 0, 9, "starts"), (300, 16, 64, 1500, 1, 128, "starts"),
+    (513, 48, 1, 700, 0, 3, "starts"), (64, 64, 0, 900, 0, -1, "whole"), (3, 1, 0, 50, 0, -1, "whole"), (4096, 128, 1, 300, 1, 1, "uniform"), (16384, 16, 1, 20, 0, 2, "starts")])
+def test_plan_matches_the_plain_form(B, page, lo, hi, new_lo, new_hi, mode):
+    lens, new, table, free = _plan_case(np.random.default_rng(B), B, page, lo, hi, new_lo, new_hi, spare=3, extra_cols=2)
+    if mode == "uniform":
+        new[:] = new[0]
+        lens = np.maximum(lens, new)
+        held = -(-(lens - new) // page)
+        total = int((-(-lens // page) - held).sum())
+        table = np.full_like(table, -7)
+        for b in range(B):
+            table[b, :held[b]] = np.arange(held[b]) + 1000 * b
+        free = np.random.default_rng(7).permutation(total + 3).astype(np.int32)
+    T = int(new.sum()) + 5   # rows behind the last token
+    want = plan64(lens, new, table, page, T, free)
+    got = _run_plan(lens, new, table, page, T, free, mode)
+    assert (got[0] == want[0]).all() and (got[1] == want[1]).all() and got[2] == want[2]
+    # a complete table: the same slots, nothing written
+    again = _run_plan(lens, new, want[0], page, T, None, mode)
+    assert (again[0] == want[0]).all() and (again[1] == want[1]).all() and again[2] is None
+
+
+@gpu
+def test_plan_when_pages_run_out_or_the_table_is_too_narrow():
+    lens, new, table, free = _plan_case(np.random.default_rng(3), 9, 16, 20, 90, 5, 60)
+    for n_free in (0, 1, len(free) // 2):
+        want = plan64(lens, new, table, 16, int(new.sum()), free[:n_free])
+        got = _run_plan(lens, new, table, 16, int(new.sum()), free[:n_free], "starts")
+        assert (got[0] == want[0]).all() and (got[1] == want[1]).all() and got[2] == want[2] > n_free
+    narrow = np.ascontiguousarray(table[:, :3])
+    want = plan64(lens, new, narrow, 16, int(new.sum()), free)
+    got = _run_plan(lens, new, narrow, 16, int(new.sum()), free, "starts")
+    assert (got[0] == want[0]).all() and (got[1] == want[1]).all() and got[2] == want[2] and (want[1] == -1).any()
+
+
+@gpu
+def test_plan_odd_inputs():
+    # more new tokens than stored ones, a request of length zero, one below zero, starts behind the token axis
+    lens, new = np.array([3, 0, -4, 33]), np.array([5, 0, 0, 2])
+    table, free = np.full((4, 4), -7, np.int32), np.arange(50, 60, dtype=np.int32)
+    table[3, :2] = (8, 9)
+    for T in (0, 4, 7, 9):
+        want = plan64(lens, new, table, 16, T, free)
+        got = _run_plan(lens, new, table, 16, T, free, "starts")
+        assert (got[0] == want[0]).all() and (got[1] == want[1]).all() and got[2] == want[2], T
+    # no request at all
+    got = _run_plan(lens[:0], new[:0], table[:0], 16, 3, free, "starts")
+    assert (got[1] == -1).all() and got[2] == 0
+    # starts that do not begin at zero, and a strided table inside a wider one whose other rows and columns stay
+    big = torch.full((6, 10), -7, dtype=torch.int32, device="cuda")
+    bt = big[1:, 2:6]
+    bt[0, 0] = 4
+    starts = torch.tensor([2, 3, 5], dtype=torch.int32, device="cuda")
+    slots, taken = uq_cuda.plan_step(torch.tensor([17, 2], device="cuda"), starts, bt, 16, 6, free_pages=torch.tensor([11, 12], dtype=torch.int32, device="cuda"))
+    assert slots.tolist() == [-1, -1, 11 * 16, 12 * 16, 12 * 16 + 1, -1] and int(taken) == 2
+    want = torch.full((6, 10), -7, dtype=torch.int32)
+    want[1, 2], want[1, 3], want[2, 2] = 4, 11, 12
+    assert torch.equal(big.cpu(), want)
+
+
+@gpu
+def test_plan_refuses_in_python():
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    for kw in (dict(new=0), dict(new=i(5)), dict(bt=i(3, 2).long()), dict(bt=i(1, 2)), dict(page=0), dict(T=-1), dict(free=i(4).long()), dict(free=i(8)[::2]), dict(bt=i(2, 3).t()),
+               dict(slots=torch.zeros(3, dtype=torch.int32, device="cuda"))):
+        a = dict(new=1, bt=i(2, 2), page=16, T=2, free=None, slots=None, **{}) | kw
+        with pytest.raises(RuntimeError):
+            uq_cuda.plan_step(i(2), a["new"], a["bt"], a["page"], a["T"], free_pages=a["free"], slots=a["slots"])
+
+
+# ------------------------------------------------------------------------------------------------------- norm and gate
+def _rand(shape, dtype, seed, size=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    chan = torch.exp(0.5 * torch.randn(shape[-1], generator=g, device="cuda"))
+    return (torch.randn(*shape, generator=g, device="cuda") * chan * size).to(dtype)
+
+
+def _f64(t):
+    return t.double().cpu().numpy()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("R,H,residual,weight", [(1, 32, True, True), (3, 64, False, True), (7, 256, True, False), (5, 288, True, True), (130, 512, True, True), (2, 1024, False, False),
+                                                 (9, 1056, True, True), (8, 8192, True, True), (3, 11040, True, True), (2, 16384, False, True), (2, 32768, True, True), (700, 4096, True, True)])
+def test_norm_matches_the_plain_form(dtype, R, H, residual, weight):
+    dt = DT[dtype]
+    x, r = _rand((R, H), dt, 1), _rand((R, H), dt, 2, 4.0) if residual else None
+    w = (1 + 0.1 * _rand((H,), torch.float32, 3)).to(dt) if weight else None
+    codes, scales, s = uq_cuda.rms_norm_mx8(x, w, r, eps=1e-5)
+    s64 = _f64(x) + (_f64(r) if residual else 0)
+    y = s64 / np.sqrt((s64 ** 2).mean(-1, keepdims=True) + 1e-5) * (_f64(w) if weight else 1)
+    check_mx8(codes, scales, y)
+    if residual:
+        assert (np.abs(_f64(s) - s64) <= (torch.finfo(dt).eps / 2 + 2.0 ** -24) * np.abs(s64) + torch.finfo(dt).tiny).all()
+    else:
+        assert s is None
+
+
+@gpu
+def test_norm_in_place_strided_and_batched():
+    x, r, w = _rand((6, 5, 96), torch.bfloat16, 1), _rand((6, 5, 96), torch.bfloat16, 2), _rand((96,), torch.bfloat16, 3)
+    want = uq_cuda.rms_norm_mx8(x, w, r)
+    assert want[0].shape == (6, 5, 96) and want[1].shape == (6, 5, 3) and want[2].shape == (6, 5, 96)
+    # rows of a wider tensor, a weight off its 16-byte boundary
+    wide = torch.zeros(6, 5, 200, dtype=torch.bfloat16, device="cuda")
+    wide[..., 3:99] = x
+    off = torch.cat([w[:1], w])[1:]
+    got = uq_cuda.rms_norm_mx8(wide[..., 3:99], off, r)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+    for target in (r, x):   # the sum into the residual's or the input's own memory
+        mine = target.clone()
+        args = (mine, w, r) if target is x else (x, w, mine)
+        got = uq_cuda.rms_norm_mx8(*args, sum_out=mine)
+        assert got[2] is mine and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+    # outputs given: rows behind them stay as they were
+    c, s = torch.full((8, 5, 96), 1.0, device="cuda").to(torch.float8_e4m3fn), torch.full((8, 5, 3), 9, dtype=torch.uint8, device="cuda")
+    uq_cuda.rms_norm_mx8(x, w, r, codes=c[:6], scales=s[:6])
+    assert torch.equal(c[:6].view(torch.uint8), want[0].view(torch.uint8)) and (c[6:].float() == 1).all() and (s[6:] == 9).all() and torch.equal(s[:6], want[1])
+    # no rows
+    got = uq_cuda.rms_norm_mx8(x[:0], w, r[:0])
+    assert got[0].shape == (0, 5, 96)
+
+
+@gpu
+@pytest.mark.parametrize("H", [64, 2048])
+def test_norm_extremes(H):
+    """Zeros, one large value, groups at and around a scale's border, values whose squares leave fp32, NaN and infinity."""
+    x = _rand((9, H), torch.float32, 5)
+    x[0] = 0
+    x[1] = 0
+    x[1, 33] = 1e-3
+    x[2] *= 1e25
+    x[3] *= 1e-30
+    x[4, :32] = 0
+    x[5] = 1.0
+    x[6] = torch.where(torch.arange(H, device="cuda") % 2 == 0, 3.0e38, -1.0e30)
+    x[7, 5] = float("nan")
+    x[8, 5] = float("inf")
+    w = torch.ones(H, device="cuda")
+    w[:32] = 448.0   # x[5]: y = 448 / sqrt(1 + eps), under the border by eps / 2 ~ 2^-11
+    codes, scales, _ = uq_cuda.rms_norm_mx8(x, w, eps=1e-3)
+    x64 = _f64(x)[:7]
+    check_mx8(codes[:7], scales[:7], x64 / np.sqrt((x64 ** 2).mean(-1, keepdims=True) + 1e-3) * _f64(w))
+    assert (codes[0].float() == 0).all() and (scales[0] == 0).all() and codes[7].float().isnan().all()
+    assert codes[8, 5].float().isnan() and (codes[8].float().nan_to_num(0) == 0).all()   # s * (1 / inf)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("R,F", [(1, 32), (3, 96), (64, 2048), (5, 2080), (33, 11040), (2, 32768)])
+def test_silu_matches_the_plain_form(dtype, R, F):
+    x = _rand((R, 2 * F), DT[dtype], R, 3.0)
+    codes, scales = uq_cuda.silu_mul_mx8(x)
+    g, u = _f64(x)[:, :F], _f64(x)[:, F:]
+    check_mx8(codes, scales, g / (1 + np.exp(-g)) * u)
+
+
+@gpu
+def test_silu_extremes():
+    g = torch.tensor([0.0, -0.0, 1e-30, -80.0, -87.0, 80.0, 1e20, -60.0], device="cuda").repeat(8).view(1, 64)
+    u = torch.tensor([1.0, -1.0, 3.0, 2.0, 5.0, -7.0, 1e5, 1e10], device="cuda").repeat_interleave(8).view(1, 64)
+    codes, scales = uq_cuda.silu_mul_mx8(torch.cat([g, u], 1))
+    g64, u64 = _f64(g), _f64(u)
+    check_mx8(codes, scales, g64 / (1 + np.exp(-g64)) * u64)
+    x = torch.ones(2, 128, device="cuda")
+    x[0, 3], x[1, 40], x[0, 64 + 50] = float("nan"), float("inf"), float("-inf")
+    codes, scales = uq_cuda.silu_mul_mx8(x)
+    bad = codes.float().isnan()
+    assert bad.sum() == 3 and bad[0, 3] and bad[1, 40] and bad[0, 50]
+    assert (codes[0, :32].float()[torch.arange(32) != 3] > 0).all()   # the NaN's neighbours keep their values
+
+
+@gpu
+def test_row_operators_refuse_in_python():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: uq_cuda.rms_norm_mx8(x[:, :48]), lambda: uq_cuda.rms_norm_mx8(x.double()), lambda: uq_cuda.rms_norm_mx8(x, x[0].float()), lambda: uq_cuda.rms_norm_mx8(x, x[0], x[:2]),
+                 lambda: uq_cuda.rms_norm_mx8(x, x[0], eps=0), lambda: uq_cuda.rms_norm_mx8(x, x[0], sum_out=x), lambda: uq_cuda.rms_norm_mx8(x, codes=x), lambda: uq_cuda.silu_mul_mx8(x[:, :32]),
+                 lambda: uq_cuda.silu_mul_mx8(x, scales=torch.zeros(4, 2, dtype=torch.uint8, device="cuda")), lambda: uq_cuda.pack_fp4_weight(x[:, :40]), lambda: uq_cuda.pack_fp4_weight(x.double())):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+# -------------------------------------------------------------------------------------------------------------- linear
+def _weight(N, K, seed, dtype=torch.float32):
+    return uq_cuda.pack_fp4_weight(_rand((N, K), dtype, seed, K ** -0.5))
+
+
+@gpu
+@pytest.mark.parametrize("N,K,rule", [(1, 32, "ceil"), (200, 160, "ceil"), (256, 384, "paper")])
+def test_pack_is_the_caches_encoder(N, K, rule):
+    w = _rand((N, K), torch.bfloat16, 4)
+    wc, ws = uq_cuda.pack_fp4_weight(w, rule=rule)
+    ref = torch.nn.functional.pad(w, (0, -K % 128)).view(N, -1, 128)
+    code, scale = torch.zeros(N, ref.shape[1], 1, 64, dtype=torch.uint8, device="cuda"), torch.zeros(N, ref.shape[1], 1, 4, dtype=torch.uint8, device="cuda")
+    uq_cuda.quantize_on_write(ref, code, scale, torch.arange(N, device="cuda"), rule)
+    rows = lambda t: t.transpose(1, 2).reshape(t.shape[0] * t.shape[2], -1)[:N]
+    assert torch.equal(rows(wc), rows(code)) and torch.equal(rows(ws), rows(scale))
+    assert (wc.transpose(1, 2).reshape(-1, wc.shape[1] * 64)[N:] == 0).all()
+
+
+SHAPES = [(1, 128, 128), (1, 1, 32), (2, 130, 160), (8, 256, 1024), (5, 1000, 1120), (17, 640, 4096), (33, 257, 96), (64, 384, 2048), (65, 129, 288), (127, 512, 256), (128, 300, 512), (130, 256, 640), (300, 128, 224)]
+
+
+@gpu
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_linear_mx8_matches_the_plain_form(M, N, K, out):
+    wc, ws = _weight(N, K, N)
+    codes, scales, _ = uq_cuda.rms_norm_mx8(_rand((M, K), torch.float32, M))
+    y = uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales, out_dtype=DT[out])
+    assert y.shape == (M, N) and y.dtype == DT[out]
+    check_linear(y, mx8_values(codes, scales), weight64(wc, ws, N, K), DT[out])
+
+
+@gpu
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_linear_bf16_matches_the_plain_form(M, N, K, out):
+    wc, ws = _weight(N, K, N + 1)
+    x = _rand((M, K), torch.bfloat16, M)
+    y = uq_cuda.fp4_linear(x, wc, ws, N, out_dtype=DT[out])
+    check_linear(y, _f64(x), weight64(wc, ws, N, K), DT[out], split=True)
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 8192), (3, 2048, 32768), (40, 20000, 1024), (16, 1024, 16384)])
+def test_linear_long_and_wide(M, N, K):
+    wc, ws = _weight(N, K, 5, torch.bfloat16)
+    x = _rand((M, K), torch.bfloat16, 6)
+    w64 = weight64(wc, ws, N, K)
+    check_linear(uq_cuda.fp4_linear(x, wc, ws, N, out_dtype=torch.float32), _f64(x), w64, torch.float32, split=True)
+    codes, scales, _ = uq_cuda.rms_norm_mx8(x)
+    check_linear(uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales), mx8_values(codes, scales), w64, torch.bfloat16)
+
+
+@gpu
+def test_linear_every_code_and_scale():
+    """All sixteen codes against all 256 e4m3 values, and scales over the whole range that products of fp32 hold."""
+    wc = torch.arange(256, dtype=torch.uint8, device="cuda").repeat(1, 1, 32, 1).view(1, 1, 128, 64).contiguous()
+    ws = torch.full((1, 1, 128, 4), 127, dtype=torch.uint8, device="cuda")
+    ws[0, 0, :, 0] = torch.arange(128, dtype=torch.uint8, device="cuda") + 60
+    ws[0, 0, :, 2] = 200
+    x = torch.zeros(254, 128, device="cuda")
+    every = torch.tensor([b for b in range(256) if b & 127 != 127], dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    codes = x.to(torch.float8_e4m3fn)
+    codes[:, 0] = every
+    codes[:, 71] = every
+    scales = torch.full((254, 4), 127, dtype=torch.uint8, device="cuda")
+    scales[:, 0] = 100
+    scales[:, 2] = torch.arange(254, dtype=torch.uint8, device="cuda") // 4 + 30
+    y = uq_cuda.fp4_linear(codes, wc, ws, scales=scales, out_dtype=torch.float32)
+    check_linear(y, mx8_values(codes, scales), weight64(wc, ws, 128, 128), torch.float32)
+
+
+@gpu
+def test_linear_rows_do_not_touch_each_other_and_nothing_beyond_is_written():
+    N, K = 200, 288
+    wc, ws = _weight(N, K, 9)
+    x = _rand((20, K), torch.bfloat16, 9)
+    want = uq_cuda.fp4_linear(x, wc, ws, N)
+    x[3, 7], x[11, 280], x[19, 0] = float("nan"), float("inf"), float("-inf")
+    buf = torch.full((24, N), 5.0, dtype=torch.bfloat16, device="cuda")
+    got = uq_cuda.fp4_linear(x, wc, ws, N, out=buf[2:22])   # (2 * 200 * 2 bytes: on its 16-byte boundary)
+    bad = torch.zeros(20, dtype=torch.bool, device="cuda")
+    bad[[3, 11, 19]] = True
+    assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad]) and (buf[:2] == 5).all() and (buf[22:] == 5).all()
+    codes, scales, _ = uq_cuda.rms_norm_mx8(x)
+    assert uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales)[3].isnan().all()
+    # zero rows and zero values
+    assert uq_cuda.fp4_linear(x[:0], wc, ws, N).shape == (0, N)
+    assert (uq_cuda.fp4_linear(torch.zeros(2, 3, K, dtype=torch.bfloat16, device="cuda"), wc, ws, N) == 0).all()
+
+
+@gpu
+def test_linear_small_and_large_values():
+    """bf16 values at both ends of the type's range: their groups' scales reach the lower end of the byte (the weight is large, so
+    that the products stay clear of fp32's subnormals)."""
+    N, K = 128, 128
+    wc, ws = _weight(N, K, 2)
+    ws += 20
+    x = _rand((4, K), torch.float32, 2)
+    x = (x * torch.tensor([1e-36, 1e-39, 1e25, 1.0], device="cuda")[:, None]).bfloat16()
+    w64 = weight64(wc, ws, N, K)
+    y = uq_cuda.fp4_linear(x, wc, ws, N, out_dtype=torch.float32)
+    x64 = _f64(x)
+    want = x64 @ w64.T
+    A = np.abs(x64) @ np.abs(w64).T
+    # beside the usual: at a scale of 2^-127 a plane's last step is 2^-136
+    assert (np.abs(_f64(y) - want) <= 2.0 ** -16 * A + 2.0 ** -135 * np.abs(w64).sum(1)).all()
+
+
+@gpu
+def test_linear_refuses_in_python():
+    wc, ws = _weight(200, 288, 1)
+    x = torch.zeros(4, 288, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: uq_cuda.fp4_linear(x.half(), wc, ws), lambda: uq_cuda.fp4_linear(x[:, :256], wc, ws), lambda: uq_cuda.fp4_linear(x, wc, ws, 300), lambda: uq_cuda.fp4_linear(x, wc, ws, 128),
+                 lambda: uq_cuda.fp4_linear(x, wc, ws[:, :2].contiguous()), lambda: uq_cuda.fp4_linear(x, wc, ws, scales=torch.zeros(4, 9, dtype=torch.uint8, device="cuda")),
+                 lambda: uq_cuda.fp4_linear(x, wc, ws, 200, out=torch.zeros(4, 256, device="cuda")), lambda: uq_cuda.fp4_linear(x, wc, ws, out_dtype=torch.float64),
+                 lambda: uq_cuda.fp4_linear(x, wc, ws, 200, workspace=torch.zeros(10, dtype=torch.uint8, device="cuda"))):
+        with pytest.raises(RuntimeError):
+            call()
