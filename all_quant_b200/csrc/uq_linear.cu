@@ -2,66 +2,355 @@
 // verify step.  No counterpart in the reference.
 //
 // The weight is laid out as one stream of the paged cache with 128-token pages at head_dim 128 (codes [tiles, K/128, 128, 64],
-// scales [tiles, K/128, 128, 4]: a tile is 128 output channels, a "head" 128 input channels), so the cache's own encoder writes it.
+// scales [tiles, K/128, 128, 4]: a tile is 128 output channels, a "head" 128 input channels), so the cache's own encoder writes it
+// and every 128 x 128 block is 8 KB of codes and 512 bytes of scales, both contiguous.
 // Activations are e4m3 codes with one UE8M0 scale per 32 channels; bf16 rows are split into two such planes first (uq_rows.cu),
 // whose products are added.
+//
+// What bounds it: reading the weight, N * K * 17 / 32 bytes, up to about 128 rows; so nothing is decoded by threads.  The block-scaled
+// tensor instruction (kind::mxf8f6f4, one UE8M0 scale per 32 elements of K) takes the weight's codes and scale bytes as they are,
+// with the 128 output channels as its M and the rows of x as its N:
+//
+//   y^T[n, m] += W[n, k] * X[m, k]     M = 128 channels, N = NB in {16, 32, 64, 128} rows, K = 32 per instruction
+//
+// The copy engine unpacks the 4-bit codes on the way into shared memory (16 codes = 8 bytes, then 8 bytes of padding: 128 codes
+// are one 128-byte row of the swizzled tile).  The instruction wants the scales of rows l, 32 + l, 64 + l, 96 + l beside one another,
+// the layout has those of 4 l .. 4 l + 3: the tensor map therefore brings the rows in the order 4 l + j -> 32 j + l (two
+// dimensions of 32 and 4 rows, the outer one first in memory), and the scale bytes are copied as they lie.
+//
+// One CTA per (128 channels, NB rows, range of K); the ranges of one tile are a cluster, whose CTAs lay their fp32 partial tiles out
+// in shared memory and add each other's up in the order of their ranks, each a share of the rows: one launch, no scratch, the same
+// bits every time.  Two CTAs fit an SM, so that their copies overlap and a grid need not be a multiple of the SMs.
 #include <climits>
 
-#include "uq_common.cuh"
+#include <algorithm>
+#include <atomic>
 
-namespace {
+#include "uq_sm100.cuh"
 
-constexpr int kSplitRows = 64;   // rows of bf16 activations in one tile of planes
+namespace tc {
 
-struct LinearArgs {
-  const uint8_t *x, *xs, *wc, *ws;
+constexpr int kThreads = 7 * 32;   // warps 0-3: scales of x, then the epilogue; 4: copies of the weight; 5: instructions; 6: copies of x and of the weight's scales
+constexpr int kWarpW = 4, kWarpMma = 5, kWarpX = 6;
+constexpr int kMaxSplit = 8;       // CTAs of a cluster
+
+struct LinearParams {
+  const uint8_t* xs;    // [rows of the x map, K / 32]
+  const uint8_t* wc;
+  const uint8_t* ws;
   void* out;
-  long long M;
-  int N, K, ksteps;
-  int planes, tile_rows;   // 1: x is [M, K]; 2: the planes that uq_split_kernel writes, tiles of tile_rows
+  unsigned int* status;
+  long long M, xrows;
+  int N, K, ksteps, mtiles;
   int out_dtype;
+  int words;            // x's scale bytes of 128 channels are aligned words
+  int pdl;
 };
 
-UQ_DEV float e4m3_byte(uint32_t b) { return uq_e4m3_f32(b & 0xffu); }
+template <int NB, int PLANES>
+struct LinCfg {
+  static constexpr int kRows = NB / PLANES;                  // rows of x per CTA
+  static constexpr int kStages = NB <= 32 ? 5 : (NB == 64 ? 4 : 3);   // what half an SM's shared memory holds
+  static constexpr int kA = 128 * 128, kB = NB * 128, kSf = 512;
+  static constexpr int oB = kA, oSfa = oB + kB, oSfb = oSfa + kSf, kStage = oSfb + kSf;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kPRow = 160;                          // floats of one row of the partial tile, see below
+  static constexpr int kP = kRows * kPRow * 4;
+  static constexpr int kBody = (kRing > kP ? kRing : kP) / 1024 * 1024 + 1024;
+  static constexpr int oBarW = kBody, oBarX = oBarW + 8 * kStages, oBarS = oBarX + 8 * kStages, oBarE = oBarS + 8 * kStages, oBarDone = oBarE + 8 * kStages;
+  static constexpr int oTmem = oBarDone + 8, oAbort = oTmem + 4;
+  static constexpr int kSmem = oAbort + 4;
+  static constexpr int cSf = NB;                             // first column of the scales: 8 per stage (4 of the weight, 4 of x)
+  static constexpr int kColsUsed = cSf + 8 * kStages;
+  static constexpr int kCols = kColsUsed <= 64 ? 64 : (kColsUsed <= 128 ? 128 : 256);   // two CTAs' share an SM's 512
+  // The ring's stages start on 1024-byte boundaries as long as a stage is a multiple of 1024 bytes (the swizzled tiles need it).
+  static_assert(kStage % 1024 == 0 && kB % 1024 == 0, "swizzled tiles sit on 1024-byte boundaries");
+  static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs per SM");
+};
 
-// A warp per output channel, 8 input channels per lane at a time.
-__global__ void __launch_bounds__(128) uq_fp4_linear_kernel(LinearArgs a, int pdl) {
-  uq_pdl_wait();
-  if (pdl) uq_pdl_release();
-  const int lane = threadIdx.x & 31;
-  const long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (n >= a.N) return;
-  for (long long m = blockIdx.y; m < a.M; m += gridDim.y) {
-    float acc = 0.f;
-    for (int k = lane * 8; k < a.K; k += 256) {
-      const size_t row = ((size_t)(n / 128) * a.ksteps + k / 128) * 128 + n % 128;
-      const uint32_t c = *reinterpret_cast<const uint32_t*>(a.wc + row * 64 + (k % 128) / 2);
-      const float wscale = uq_scale_f32(a.ws[row * 4 + (k % 128) / 32]);
-      for (int pl = 0; pl < a.planes; pl++) {
-        long long xr = m;
-        if (a.planes == 2) {
-          const long long tile = m / a.tile_rows, left = a.M - tile * a.tile_rows;
-          xr = tile * 2 * a.tile_rows + m % a.tile_rows + (pl ? (min(left, (long long)a.tile_rows) + 7) / 8 * 8 : 0);
+// shared-memory matrix descriptor without a swizzle, for the copy of 32 rows of 16 bytes (8-row groups 128 bytes apart)
+UQ_DEV uint64_t sf_desc(uint32_t addr) { return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46); }
+// 32 rows of 16 bytes -> 4 columns of the 32 lanes, the same in all four lane quarters; ordered with this thread's tensor instructions
+UQ_DEV void tmem_copy_sf(uint32_t taddr, uint64_t desc) { asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory"); }
+UQ_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x0, int x1, int x2, int x3, uint32_t bar, uint64_t pol) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;"
+               ::"r"(dst), "l"(map), "r"(x0), "r"(x1), "r"(x2), "r"(x3), "r"(bar), "l"(pol) : "memory");
+}
+UQ_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+UQ_DEV uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+UQ_DEV float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int NB, int PLANES>
+__global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid_constant__ LinearParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+  using C = LinCfg<NB, PLANES>;
+  extern __shared__ __align__(1024) uint8_t smem_lin[];
+  const uint32_t sm = smem_u32(smem_lin);
+  if (sm & 1023u) {   // never expected; the swizzled layouts below would be wrong
+    uq_pdl_wait();
+    if (threadIdx.x == 0) uq_report(p.status, 2u, sm, 1u);
+    return;           // (every CTA of a cluster alike: the offset is the kernel's)
+  }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = gridDim.y, rank = blockIdx.y;
+  const int tile_n = blockIdx.x / p.mtiles, tile_m = blockIdx.x % p.mtiles;
+  const int k0 = (int)((long long)p.ksteps * rank / split), nk = (int)((long long)p.ksteps * (rank + 1) / split) - k0;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_lin + C::oAbort);
+  auto stage_at = [&](int s) { return sm + s * C::kStage; };
+  auto bar = [&](int o, int s) { return sm + o + 8 * s; };
+  auto wait = [&](uint32_t b, uint32_t parity, int id, int k) -> bool {
+    bool r = mbar_test(b, parity);
+    if (!r) r = mbar_try(b, parity);
+    if (!r) r = bounded_wait(b, parity, abort_flag, p.status, id, k);
+    return r;
+  };
+  const size_t block0 = (size_t)tile_n * p.ksteps + k0;   // first 128 x 128 block of this CTA's range
+  constexpr int kScaleWarps = (NB + 31) / 32;
+
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; s++) {
+      mbar_init(bar(C::oBarW, s), 1);
+      mbar_init(bar(C::oBarX, s), 1);
+      mbar_init(bar(C::oBarS, s), kScaleWarps);
+      mbar_init(bar(C::oBarE, s), 1);
+    }
+    mbar_init(bar(C::oBarDone, 0), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    // The first blocks of the weight on their way into L2 while the kernel before this one still runs: a hint that reads nothing -
+    // should that kernel write the weight, the lines in L2 are what it writes.
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.wc + block0 * 8192), "r"(min(nk, C::kStages) * 8192) : "memory");
+  }
+  uq_pdl_wait();   // from here on global memory is read and written
+  if (p.pdl) uq_pdl_release();
+  if (warp == kWarpMma) {   // (after the wait: see the verify kernel)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm + C::oTmem), "n"(C::kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
+
+  if (warp == kWarpW || warp == kWarpX) {
+    // ---- copies: one thread each for the weight's codes, and for x with the weight's scales (a copy costs its thread some 300 cycles)
+    if (elect_one()) {
+      const bool weights = warp == kWarpW;
+      const uint64_t pol = l2_policy();
+      uint64_t keep;
+      asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
+      const int full = weights ? C::oBarW : C::oBarX;
+      int i = 0;
+      bool ok = true;
+      for (; i < nk; i++) {
+        const int s = i % C::kStages;
+        if (i >= C::kStages && !(ok = wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 40, i))) break;
+        const uint32_t st = stage_at(s), b = bar(full, s);
+        if (weights) {
+          mbar_expect_tx(b, 8192);   // the packed bytes are counted
+          tma_load_4d(st, &map_w, 0, 0, 0, (int)(block0 + i), b, pol);
+        } else {
+          mbar_expect_tx(b, C::kB + C::kSf);
+          tma_load_2d(st + C::oB, &map_x, (k0 + i) * 128, tile_m * NB, b, keep);
+          bulk_load(st + C::oSfa, p.ws + (block0 + i) * 512, 512, b, pol);
         }
-        const uint2 v = *reinterpret_cast<const uint2*>(a.x + xr * a.K + k);
-        float part = 0.f;
-        for (int i = 0; i < 8; i++) part = fmaf(e4m3_byte((i < 4 ? v.x : v.y) >> (8 * (i & 3))), uq_e2m1_f32((c >> (4 * i)) & 15u), part);
-        acc = fmaf(part * uq_scale_f32(a.xs[xr * (a.K / 32) + k / 32]), wscale, acc);
+      }
+      if (!ok)   // gave up: what this thread still has in flight lands before the CTA may end
+        for (int j = max(i - C::kStages, 0); j < i; j++) bounded_wait(bar(full, j % C::kStages), (j / C::kStages) & 1, abort_flag, p.status, 41, j);
+    }
+  } else if (warp == kWarpMma) {
+    if (elect_one()) {
+      bool ok = true;
+      for (int i = 0; i < nk && ok; i++) {
+        const int s = i % C::kStages;
+        const uint32_t parity = (i / C::kStages) & 1;
+        ok = wait(bar(C::oBarX, s), parity, 42, i) && wait(bar(C::oBarS, s), parity, 43, i) && wait(bar(C::oBarW, s), parity, 44, i);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t st = stage_at(s), sf = tmem + C::cSf + 8 * s;
+        tmem_copy_sf(sf, sf_desc(st + C::oSfa));
+        tmem_copy_sf(sf + 4, sf_desc(st + C::oSfb));
+        const uint64_t a = smem_desc(st, 16, 1024), b = smem_desc(st + C::oB, 16, 1024);
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++)
+          mma_bs(tmem, a + (uint64_t)(kb * 2), b + (uint64_t)(kb * 2), instr_desc_bs(128, NB, 5, 0, kb, kb), sf, sf + 4, (i || kb) ? 1u : 0u);
+        tc_commit(bar(C::oBarE, s));
+      }
+      if (ok) tc_commit(bar(C::oBarDone, 0));
+    }
+  } else {
+    // ---- x's scales: thread r has row r's four bytes of every 128 channels, four loads ahead
+    if (warp < kScaleWarps) {
+      const int groups = p.K / 32;
+      const long long row = (long long)tile_m * NB + tid;
+      const bool have = tid < NB && row < p.xrows;
+      const uint8_t* src = p.xs + row * groups;
+      auto load = [&](int i) -> uint32_t {
+        uint32_t w = 0x7f7f7f7fu;
+        if (have && i < nk) {
+          const int g = (k0 + i) * 4;
+          if (p.words) return *reinterpret_cast<const uint32_t*>(src + g);
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (g + j < groups) w = (w & ~(0xffu << (8 * j))) | ((uint32_t)src[g + j] << (8 * j));
+        }
+        return w;
+      };
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = load(j);
+      bool ok = true;
+      for (int i0 = 0; i0 < nk && ok; i0 += 4) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int i = i0 + j;
+          if (i >= nk || !ok) break;
+          const int s = i % C::kStages;
+          if (i >= C::kStages) ok = __all_sync(0xffffffffu, wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 45, i));
+          if (!ok) break;
+          if (tid < NB) *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfb + lane * 16 + warp * 4) = w[j];
+          w[j] = load(i + 4);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::oBarS, s));
+        }
       }
     }
-    for (int d = 16; d; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
-    if (lane == 0) {
-      const size_t o = (size_t)m * a.N + n;
-      if (a.out_dtype == 0) static_cast<float*>(a.out)[o] = acc;
-      else if (a.out_dtype == 1) static_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16(acc);
-      else static_cast<__half*>(a.out)[o] = __float2half(acc);
+    // ---- epilogue, first half: the accumulator's lane 32 j + l is channel 4 l + j of the tile.  A row of the partial tile is four runs
+    // of 32 floats, 40 apart: its writers (a run per warp) and its readers (consecutive channels) both meet every bank once.
+    if (wait(bar(C::oBarDone, 0), 0, 46, nk)) {
+      tc_fence_after();
+      float* part = reinterpret_cast<float*>(smem_lin) + warp * 40 + lane;
+#pragma unroll
+      for (int c = 0; c < C::kRows; c += 8) {
+        uint32_t v[8];
+        tmem_ld8(tmem + ((uint32_t)(warp * 32) << 16) + c, v);
+        if (PLANES == 2) {
+          uint32_t u[8];
+          tmem_ld8(tmem + ((uint32_t)(warp * 32) << 16) + C::kRows + c, u);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u[j]));
+        } else {
+          tc_wait_ld();
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) part[(c + j) * C::kPRow] = __uint_as_float(v[j]);
+      }
+      tc_fence_before();
     }
+  }
+  __syncthreads();
+  if (*abort_flag) {   // (the copies in flight have been waited for) the failure shows in the output
+    for (int i = tid; i < C::kRows * C::kPRow; i += kThreads) reinterpret_cast<float*>(smem_lin)[i] = __int_as_float(0x7fc00000);
+  }
+  if (split > 1) cluster_sync(); else __syncthreads();
+  // ---- second half: this CTA's share of the rows, the partial tiles in the order of the ranks
+  if (tid < 128) {
+    const int n = tile_n * 128 + tid;
+    const long long m0 = (long long)tile_m * C::kRows;
+    const int rows = (int)min((long long)C::kRows, p.M - m0);
+    const uint32_t at = sm + ((tid & 3) * 40 + (tid >> 2)) * 4;
+    if (n < p.N)
+      for (int t = rank; t < rows; t += split) {
+        float v = 0.f;
+        if (split == 1) {
+          v = *reinterpret_cast<const float*>(smem_lin + (at - sm) + t * C::kPRow * 4);
+        } else {
+          for (int r = 0; r < split; r++) v += ld_cluster(cluster_addr(at + t * C::kPRow * 4, r));
+        }
+        const size_t o = (size_t)(m0 + t) * p.N + n;
+        if (p.out_dtype == 0) static_cast<float*>(p.out)[o] = v;
+        else if (p.out_dtype == 1) static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16(v);
+        else static_cast<__half*>(p.out)[o] = __float2half(v);
+      }
+  }
+  if (split > 1) cluster_sync();   // nobody leaves while its partial tile is being read
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kCols) : "memory");
   }
 }
 
+// ---------------------------------------------------------------------------------------------- host
+// The weight's codes: 128 codes of a row, rows 4 l + j of a block as (l, j), blocks.
+bool weight_map(CUtensorMap* map, const uint8_t* wc, long long blocks) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {128, 32, 4, (cuuint64_t)blocks};
+  const cuuint64_t strides[3] = {256, 64, 8192};
+  const cuuint32_t box[4] = {128, 32, 4, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 4, const_cast<uint8_t*>(wc), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// x's codes: K channels (zeros behind them), rows of which a box takes nb.
+bool x_map(CUtensorMap* map, const uint8_t* x, long long rows, int K, int nb) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)K};
+  const cuuint32_t box[2] = {128, (cuuint32_t)nb};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NB, int PLANES>
+cudaError_t linear_launch(const LinearParams& p, const uint8_t* x, int tiles, int split, cudaStream_t s) {
+  using C = LinCfg<NB, PLANES>;
+  auto kern = uq_fp4_linear_kernel<NB, PLANES>;
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) { cudaGetLastError(); return e; }
+    ready[dev].store(true, std::memory_order_release);
+  }
+  CUtensorMap mw, mx;
+  if (!weight_map(&mw, p.wc, (long long)tiles * p.ksteps) || !x_map(&mx, x, p.xrows, p.K, NB)) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)tiles * p.mtiles, (unsigned)split);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = p.pdl;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = (unsigned)split;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, mw, mx);
+  if (e != cudaSuccess) cudaGetLastError();
+  return e;
+}
+
+}  // namespace tc
+
+namespace {
+
 bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
-long long plane_rows(long long M) { return (M + kSplitRows - 1) / kSplitRows * 2 * kSplitRows; }
+// rows of an instruction's operand that serve r rows of x
+int operand_rows(long long r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ? 64 : 128)); }
+// rows of both planes of M bf16 rows: tiles of 64, one smaller tile for fewer
+int plane_tile(long long M) { return operand_rows(2 * std::min(M, 64ll)); }
+long long plane_rows(long long M) { return (M + 63) / 64 * plane_tile(M); }
 
 }  // namespace
 
@@ -73,27 +362,58 @@ size_t uq_fp4_linear_scratch(long long M, int K) { return M < 1 || K < 32 || K %
 // xs null: x is bf16 [M, K], scratch holds uq_fp4_linear_scratch bytes; else x is e4m3 [M, K] with scale bytes xs [M, K / 32].
 // launches: kernels enqueued.
 cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, void* out, void* scratch, long long M, int N, int K, int out_dtype,
-                                   unsigned int* status, cudaStream_t s, int* launches) {
+                                   unsigned int* status, int sms, cudaStream_t s, int* launches) {
   *launches = 0;
   if (M < 0 || M > (1 << 24) || N < 1 || N > (1 << 24) || K < 32 || K > (1 << 24) || K % 32 || out_dtype < 0 || out_dtype > 2) return cudaErrorInvalidValue;
   if (M == 0) return cudaSuccess;
   if (!x || !wc || !ws || !out || (!xs && !scratch)) return cudaErrorInvalidValue;
   if (!aligned_to(x, 16) || !aligned_to(wc, 32) || !aligned_to(ws, 16) || !aligned_to(out, 16) || (xs ? !aligned_to(xs, 4) : !aligned_to(scratch, 16))) return cudaErrorInvalidValue;
-  (void)status;
-  LinearArgs a{static_cast<const uint8_t*>(x), xs, wc, ws, out, M, N, K, (K + 127) / 128, 1, 0, out_dtype};
-  if (!xs) {
-    uint8_t* codes = static_cast<uint8_t*>(scratch);
-    uint8_t* scales = codes + (size_t)plane_rows(M) * K;
-    const cudaError_t e = uq_split_dispatch(x, codes, scales, M, K, kSplitRows, s);
+  const long long tiles = (N + 127) / 128, ksteps = (K + 127) / 128;
+  const int planes = xs ? 1 : 2;
+  const int nb = planes == 2 ? plane_tile(M) : operand_rows(M);
+  const long long mtiles = (M + nb / planes - 1) / (nb / planes);
+  if (tiles * ksteps > INT_MAX || tiles * mtiles > INT_MAX) return cudaErrorInvalidValue;
+  if (!status || !tc::encode_fn()) return cudaErrorInitializationError;
+  tc::LinearParams p{};
+  const uint8_t* codes = static_cast<const uint8_t*>(x);
+  p.xs = xs;
+  p.xrows = M;
+  if (planes == 2) {
+    p.xrows = plane_rows(M);
+    uint8_t* c = static_cast<uint8_t*>(scratch);
+    uint8_t* sc = c + (size_t)p.xrows * K;
+    const cudaError_t e = uq_split_dispatch(x, c, sc, M, K, nb / 2, s);
     if (e != cudaSuccess) return e;
     *launches += 1;
-    a.x = codes;
-    a.xs = scales;
-    a.planes = 2;
-    a.tile_rows = kSplitRows;
+    codes = c;
+    p.xs = sc;
   }
-  const bool pdl = uq_pdl_on();
-  const cudaError_t e = uq_launch(uq_fp4_linear_kernel, dim3((unsigned)((N + 3) / 4), (unsigned)(M < 32768 ? M : 32768)), 128u, 0, s, pdl, a, (int)pdl);
+  p.wc = wc;
+  p.ws = ws;
+  p.out = out;
+  p.status = status;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.ksteps = (int)ksteps;
+  p.mtiles = (int)mtiles;
+  p.out_dtype = out_dtype;
+  p.words = K % 128 == 0 && aligned_to(p.xs, 4);
+  p.pdl = uq_pdl_on() ? 1 : 0;
+  // CTAs along K: as many as two per SM hold, each with four steps at least
+  const long long fit = 2ll * sms / std::max(1ll, tiles * mtiles);
+  const int split = (int)std::max(1ll, std::min({(long long)tc::kMaxSplit, fit, ksteps / 4}));
+  cudaError_t e;
+  switch (nb * 2 + planes) {
+    case 33: e = tc::linear_launch<16, 1>(p, codes, (int)tiles, split, s); break;
+    case 34: e = tc::linear_launch<16, 2>(p, codes, (int)tiles, split, s); break;
+    case 65: e = tc::linear_launch<32, 1>(p, codes, (int)tiles, split, s); break;
+    case 66: e = tc::linear_launch<32, 2>(p, codes, (int)tiles, split, s); break;
+    case 129: e = tc::linear_launch<64, 1>(p, codes, (int)tiles, split, s); break;
+    case 130: e = tc::linear_launch<64, 2>(p, codes, (int)tiles, split, s); break;
+    case 257: e = tc::linear_launch<128, 1>(p, codes, (int)tiles, split, s); break;
+    default: e = tc::linear_launch<128, 2>(p, codes, (int)tiles, split, s); break;
+  }
   if (e == cudaSuccess) *launches += 1;
   return e;
 }

@@ -250,8 +250,8 @@ __global__ void __launch_bounds__(kGateThreads) uq_silu_mul_kernel(GateArgs a, i
 }
 
 // ---- split of bf16 rows into two planes -------------------------------------------------------------------------------
-// Rows are laid out as uq_linear.cu reads them: tiles of kSplitRows rows, a tile's leading planes, then its remainder planes,
-// each padded to a multiple of 8 rows (`padded`); padding rows are never written, their products never read.
+// Rows are laid out as uq_linear.cu reads them: tiles of tile_rows rows, a tile's leading planes, then its remainder planes; what
+// fills up the last tile is never written, its products never read.
 UQ_DEV void e4m3x2_to_f32(uint32_t v, float& lo, float& hi) {
   uint32_t h2;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((unsigned short)v));
@@ -265,9 +265,7 @@ __global__ void __launch_bounds__(kGateThreads) uq_split_kernel(const __nv_bfloa
   const int p = blockIdx.x * kGateThreads + threadIdx.x;
   const bool in = p < pieces;
   for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
-    const long long tile = row / tile_rows, left = rows - tile * tile_rows;
-    const int padded = (int)((min(left, (long long)tile_rows) + 7) / 8 * 8);
-    const long long hi_row = tile * 2 * tile_rows + (row - tile * tile_rows), lo_row = hi_row + padded;
+    const long long hi_row = row + row / tile_rows * tile_rows, lo_row = hi_row + tile_rows;
     float v[kPiece];
     if (in) {
       Raw<__nv_bfloat16> xr;

@@ -708,8 +708,9 @@ def fp4_linear(x, wc, ws, n=None, *, scales=None, out=None, out_dtype=None, work
 
 
 def _fp4_scratch(M, K):
-    """uqb_fp4_linear_scratch_bytes in Python: two planes per tile of 64 rows (tests/test_step_ops.py holds the two together)."""
-    return -(-M // 64) * 128 * (K + K // 32)
+    """uqb_fp4_linear_scratch_bytes in Python: two planes per tile of 64 rows, or of 8, 16 or 32 that hold all (a test holds the two together)."""
+    rows = min(M, 64)
+    return -(-M // 64) * (16 if rows <= 8 else 32 if rows <= 16 else 64 if rows <= 32 else 128) * (K + K // 32) if M > 0 else 0
 
 
 def uq_decode_partial(q, kc, ks, vc, vs, block_table, seq_lens, pos_offset=None, *, nsplit=None, sm_scale=None, workspace=None,
