@@ -44,7 +44,7 @@ cudaError_t uq_layout_dispatch(int, uint8_t*, uint8_t*, uint8_t*, uint8_t*, uint
 cudaError_t uq_merge_packed_dispatch(const float*, int, size_t, int, void*, cudaStream_t);
 cudaError_t uq_plan_dispatch(const int32_t*, const int32_t*, int, int32_t*, long long, const int32_t*, long long, int64_t*, int32_t*, int, long long, int, int, int sms, cudaStream_t);
 cudaError_t uq_rms_norm_dispatch(const void*, const void*, const void*, void*, uint8_t*, uint8_t*, long long, int, int, float, int sms, cudaStream_t);
-cudaError_t uq_silu_mul_dispatch(const void*, uint8_t*, uint8_t*, long long, int, int, cudaStream_t);
+cudaError_t uq_silu_mul_dispatch(const void*, uint8_t*, uint8_t*, long long, int, int, int sms, cudaStream_t);
 size_t uq_fp4_linear_scratch(long long, int);
 cudaError_t uq_fp4_linear_dispatch(const void*, const uint8_t*, const uint8_t*, const uint8_t*, void*, void*, long long, int, int, int, unsigned int* status, int sms, cudaStream_t, int* launches);
 
@@ -320,7 +320,7 @@ int uqb_rms_norm_mx8_launch(const void* x, const void* residual, const void* wei
 }
 
 int uqb_silu_mul_mx8_launch(const void* x, uint8_t* codes, uint8_t* scales, long long rows, int F, int dtype, void* stream) {
-  cudaError_t e = uq_silu_mul_dispatch(x, codes, scales, rows, F, dtype, reinterpret_cast<cudaStream_t>(stream));
+  cudaError_t e = uq_silu_mul_dispatch(x, codes, scales, rows, F, dtype, sm_count(), reinterpret_cast<cudaStream_t>(stream));
   if (e == cudaSuccess && rows > 0) g_launches += 1;
   return (int)e;
 }

@@ -91,6 +91,31 @@ UQ_DEV float ld_cluster(uint32_t addr) {
   return v;
 }
 
+// Four consecutive channels n.. of a row of N: one store where the rows' boundaries allow it, else those inside the row one by one.
+UQ_DEV void store4(float* o, const float* v, int n, int N) {
+  if (N % 4 == 0) {
+    if (n < N) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (n + j < N) o[j] = v[j];
+  }
+}
+UQ_DEV uint32_t pack2(float a, float b, __nv_bfloat16) { return pack_bf16x2(a, b); }
+UQ_DEV uint32_t pack2(float a, float b, __half) { return pack_f16x2(a, b); }
+template <typename T>
+UQ_DEV void store4(T* o, const float* v, int n, int N) {
+  const uint32_t a = pack2(v[0], v[1], T{}), b = pack2(v[2], v[3], T{});
+  if (N % 4 == 0) {
+    if (n < N) *reinterpret_cast<uint2*>(o) = make_uint2(a, b);
+  } else {
+    const uint32_t w[4] = {a & 0xffffu, a >> 16, b & 0xffffu, b >> 16};
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (n + j < N) reinterpret_cast<unsigned short*>(o)[j] = (unsigned short)w[j];
+  }
+}
+
 template <int NB, int PLANES>
 __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid_constant__ LinearParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
   using C = LinCfg<NB, PLANES>;
@@ -255,25 +280,38 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
     for (int i = tid; i < C::kRows * C::kPRow; i += kThreads) reinterpret_cast<float*>(smem_lin)[i] = __int_as_float(0x7fc00000);
   }
   if (split > 1) cluster_sync(); else __syncthreads();
-  // ---- second half: this CTA's share of the rows, the partial tiles in the order of the ranks
-  if (tid < 128) {
-    const int n = tile_n * 128 + tid;
+  // ---- second half: this CTA's share of the rows, the partial tiles in the order of the ranks.  A warp per row, four consecutive
+  // channels per lane; the loads of all ranks are issued before the first addition.
+  {
+    const int n = tile_n * 128 + 4 * lane;
     const long long m0 = (long long)tile_m * C::kRows;
     const int rows = (int)min((long long)C::kRows, p.M - m0);
-    const uint32_t at = sm + ((tid & 3) * 40 + (tid >> 2)) * 4;
-    if (n < p.N)
-      for (int t = rank; t < rows; t += split) {
-        float v = 0.f;
-        if (split == 1) {
-          v = *reinterpret_cast<const float*>(smem_lin + (at - sm) + t * C::kPRow * 4);
-        } else {
-          for (int r = 0; r < split; r++) v += ld_cluster(cluster_addr(at + t * C::kPRow * 4, r));
-        }
-        const size_t o = (size_t)(m0 + t) * p.N + n;
-        if (p.out_dtype == 0) static_cast<float*>(p.out)[o] = v;
-        else if (p.out_dtype == 1) static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16(v);
-        else static_cast<__half*>(p.out)[o] = __float2half(v);
+    for (int t = rank + warp * split; t < rows; t += (kThreads / 32) * split) {
+      const uint32_t at = sm + (uint32_t)(t * C::kPRow + lane) * 4;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (split == 1) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const float*>(smem_lin + (at - sm) + j * 160);
+      } else {
+        float u[kMaxSplit][4];
+#pragma unroll
+        for (int r = 0; r < kMaxSplit; r++)
+          if (r < split) {
+            const uint32_t a = cluster_addr(at, r);
+#pragma unroll
+            for (int j = 0; j < 4; j++) u[r][j] = ld_cluster(a + j * 160);
+          }
+#pragma unroll
+        for (int r = 0; r < kMaxSplit; r++)
+          if (r < split)
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] += u[r][j];
       }
+      const size_t o = (size_t)(m0 + t) * p.N + n;
+      if (p.out_dtype == 0) store4(static_cast<float*>(p.out) + o, v, n, p.N);
+      else if (p.out_dtype == 1) store4(static_cast<__nv_bfloat16*>(p.out) + o, v, n, p.N);
+      else store4(static_cast<__half*>(p.out) + o, v, n, p.N);
+    }
   }
   if (split > 1) cluster_sync();   // nobody leaves while its partial tile is being read
   if (warp == kWarpMma) {

@@ -18,7 +18,7 @@
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kTokensPerBlock = 4 * kThreads;   // tokens a block is launched for
+constexpr int kTokensPerBlock = kThreads;       // tokens a block is launched for
 constexpr int kMaxRequests = 16384;             // two prefix sums of 4 bytes in shared memory
 
 struct PlanArgs {
@@ -38,7 +38,9 @@ UQ_DEV void request(const PlanArgs& a, int b, int& len, int& n) {
   len = max(a.seq_lens[b], 0);
   n = a.K > 0 ? a.K : (a.starts ? max((int)min((long long)a.starts[b + 1] - a.starts[b], (long long)INT_MAX), 0) : len);
 }
-UQ_DEV int pages_of(long long tokens, int page, int most) { return tokens <= 0 ? 0 : (int)min((tokens + page - 1) / page, (long long)most); }
+UQ_DEV int pages_of(long long tokens, int page, int most) {   // (tokens <= INT_MAX: a 32-bit division)
+  return tokens <= 0 ? 0 : (int)min(((unsigned)tokens - 1u) / (unsigned)page + 1u, (unsigned)most);
+}
 
 // the last i with v[i] <= x, v[0..n] not decreasing and v[0] <= x
 UQ_DEV int last_not_above(const int* v, int n, int x) {
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) uq_plan_kernel(PlanArgs a, int pdl) 
       request(a, b, len, n);
       const long long pos = (long long)len - n + (t - first[b]);
       if (pos >= 0 && pos < len) {
-        const long long pi = pos / a.PAGE;
+        const int pi = (int)((unsigned)pos / (unsigned)a.PAGE);
         if (pi < a.max_pages) {
           const int held = pages_of((long long)len - n, a.PAGE, a.max_pages);
           int page = -1;
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) uq_plan_kernel(PlanArgs a, int pdl) 
             const long long at = off[b] + (pi - held);
             if (at < a.n_free) page = a.free_pages[at];
           }
-          if (page >= 0) slot = (int64_t)page * a.PAGE + (pos - pi * a.PAGE);
+          if (page >= 0) slot = (int64_t)page * a.PAGE + (pos - (long long)pi * a.PAGE);
         }
       }
     }

@@ -13,6 +13,7 @@
 //
 // All three are bound by memory: a lane owns pieces of 8 channels (one 16-byte load of a 16-bit type), a group of 32 is four
 // lanes, whose maximum takes two shuffles; a piece leaves as one 8-byte store.
+#include <atomic>
 #include <climits>
 
 #include "uq_common.cuh"
@@ -72,11 +73,27 @@ template <> struct Raw<__half> {
 };
 
 // ---- the quantiser --------------------------------------------------------------------------------------------------
+// Two operations per issue slot: these kernels run out of those first.
+UQ_DEV void mul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+UQ_DEV void add2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+UQ_DEV void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {   // d = a * b + c
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+UQ_DEV float max3(float a, float b, float c) {   // (a NaN is left out: its own code says it)
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 UQ_DEV float piece_amax(const float* v) {
-  float m = fabsf(v[0]);
-#pragma unroll
-  for (int i = 1; i < kPiece; i++) m = fmaxf(m, fabsf(v[i]));   // (a NaN is left out: its own code says it)
-  return m;
+  const float a = max3(fabsf(v[0]), fabsf(v[1]), fabsf(v[2])), b = max3(fabsf(v[3]), fabsf(v[4]), fabsf(v[5]));
+  return fmaxf(max3(a, fabsf(v[6]), fabsf(v[7])), b);
 }
 UQ_DEV float group_amax(float m) {   // over the four lanes of a group
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
@@ -95,11 +112,13 @@ UQ_DEV uint32_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
   return d;
 }
+// Codes of a piece: e4m3(v * inv), NaN where `amax`, its group's, says that there is an infinity and it is this value (the
+// conversion would saturate it).
 UQ_DEV uint2 codes_of(const float* v, float inv, float amax) {
   float q[kPiece];
 #pragma unroll
-  for (int i = 0; i < kPiece; i++) q[i] = v[i] * inv;
-  if (__float_as_uint(amax) >= 0x7f800000u) {   // an infinity in the group: the conversion would saturate it
+  for (int i = 0; i < kPiece; i += 2) mul2(q[i], q[i + 1], v[i], v[i + 1], inv, inv);
+  if (__float_as_uint(amax) >= 0x7f800000u) {
 #pragma unroll
     for (int i = 0; i < kPiece; i++) q[i] = fabsf(v[i]) <= 3.4028235e38f ? q[i] : __int_as_float(0x7fc00000);
   }
@@ -113,99 +132,121 @@ struct NormArgs {
   uint8_t *codes, *scales;
   long long rows;
   int H;
-  float eps;
+  float inv_h, eps;        // 1 / H
 };
 
-// Sum over the `lanes` threads of a row: they are `warps_row` whole warps of the block.
+// Sum over a row's threads: a warp, or the block, whose warps leave their sums in an array (zero behind the last warp).
 template <bool kOneWarp>
-UQ_DEV float row_sum(float v, float* sums, int warps_row, int first_warp) {
+UQ_DEV float row_sum(float v, float* sums) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   if (kOneWarp) return v;
   if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
   __syncthreads();
   float t = 0.f;
-  for (int i = 0; i < warps_row; i++) t += sums[first_warp + i];
-  __syncthreads();
+  for (int i = 0; i < (int)blockDim.x; i += 128) {   // four warps' sums at a time
+    const float4 q = *reinterpret_cast<const float4*>(sums + (i >> 5));
+    t += (q.x + q.y) + (q.z + q.w);
+  }
   return t;
 }
 
+UQ_DEV float inverse_root(float v) {   // (v is never subnormal: eps is not)
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // A row per block, or (kOneWarp) per warp; V pieces per lane, the row stays in registers between its two uses.
+// With t = s * w, y = t * inv and amax(y) = amax(t) * inv (a product by one factor keeps the order), so that a value costs one
+// multiplication by inv * 2^-E on its way to its code, a power of two times what y itself rounds to.
 template <typename T, int V, bool kOneWarp>
 __global__ void __launch_bounds__(kOneWarp ? 128 : 1024) uq_rms_norm_kernel(NormArgs a, int pdl) {
-  __shared__ float sums[32];
+  __shared__ __align__(16) float sums[32];
   const int lanes = kOneWarp ? 32 : blockDim.x;
   const int pieces = a.H / kPiece;
+  if (!kOneWarp && threadIdx.x < 32) sums[threadIdx.x] = 0.f;
+  if (!kOneWarp) __syncthreads();
   uq_pdl_wait();
   if (pdl) uq_pdl_release();
   const int t = kOneWarp ? (threadIdx.x & 31) : threadIdx.x;
   const long long row = kOneWarp ? (long long)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  if (kOneWarp && row >= a.rows) return;
-  const T* x = static_cast<const T*>(a.x) + row * a.H;
-  const T* r = a.r ? static_cast<const T*>(a.r) + row * a.H : nullptr;
-  const T* w = static_cast<const T*>(a.w);
+  const T *x = static_cast<const T*>(a.x), *r = static_cast<const T*>(a.r), *w = static_cast<const T*>(a.w);
   Raw<T> xr[V], rr[V];
+  if (kOneWarp && row >= a.rows) return;
+  {
+    const T *px = x + row * a.H, *pr = r + row * a.H;
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int p = t + i * lanes;
-    if (p < pieces) {
-      xr[i].load(x + (size_t)p * kPiece);
-      if (r) rr[i].load(r + (size_t)p * kPiece);
-    }
-  }
-  float s[V][kPiece];
-  float sq = 0.f;
-#pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int p = t + i * lanes;
-    if (p < pieces) {
-      xr[i].get(s[i]);
-      if (r) {
-        float o[kPiece];
-        rr[i].get(o);
-#pragma unroll
-        for (int j = 0; j < kPiece; j++) s[i][j] += o[j];
-        Raw<T>::store(static_cast<T*>(a.sum) + row * a.H + (size_t)p * kPiece, s[i]);
+    for (int i = 0; i < V; i++) {
+      const int p = t + i * lanes;
+      if (p < pieces) {
+        xr[i].load(px + p * kPiece);
+        if (r) rr[i].load(pr + p * kPiece);
       }
-      float q = 0.f;
-#pragma unroll
-      for (int j = 0; j < kPiece; j++) q = fmaf(s[i][j], s[i][j], q);
-      sq += q;
     }
   }
-  float total = row_sum<kOneWarp>(sq, sums, (lanes + 31) >> 5, 0);
-  float inv = rsqrtf(total / (float)a.H + a.eps);
-  if (__float_as_uint(total) == 0x7f800000u) {
-    // the squares left fp32 (entries beyond 2^63): once more with the row scaled by 2^-80, whose eps is nothing beside it
-    constexpr float kDown = 8.2718061255302767e-25f;   // 2^-80
-    sq = 0.f;
+  {
+    float s[V][kPiece];
+    float sq0 = 0.f, sq1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; i++)
-      if (t + i * lanes < pieces)
+    for (int i = 0; i < V; i++) {
+      const int p = t + i * lanes;
+      if (p < pieces) {
+        xr[i].get(s[i]);
+        if (r) {
+          float o[kPiece];
+          rr[i].get(o);
 #pragma unroll
-        for (int j = 0; j < kPiece; j++) sq = fmaf(s[i][j] * kDown, s[i][j] * kDown, sq);
-    total = row_sum<kOneWarp>(sq, sums, (lanes + 31) >> 5, 0);
-    inv = rsqrtf(total / (float)a.H) * kDown;
-  }
+          for (int j = 0; j < kPiece; j += 2) add2(s[i][j], s[i][j + 1], s[i][j], s[i][j + 1], o[j], o[j + 1]);
+          Raw<T>::store(static_cast<T*>(a.sum) + row * a.H + p * kPiece, s[i]);
+        }
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int p = t + i * lanes;
-    const bool in = p < pieces;
-    if (in) {
-      float wv[kPiece];
-      if (w) {
+        for (int j = 0; j < kPiece; j += 2) fma2(sq0, sq1, s[i][j], s[i][j + 1], s[i][j], s[i][j + 1], sq0, sq1);
+      }
+    }
+    float total = row_sum<kOneWarp>(sq0 + sq1, sums);
+    float inv = inverse_root(fmaf(total, a.inv_h, a.eps));
+    if (__float_as_uint(total) == 0x7f800000u) {
+      // the squares left fp32 (entries beyond 2^56): once more with the row scaled by 2^-72, whose eps is nothing beside it
+      constexpr float kDown = 2.1175823681357508e-22f;   // 2^-72
+      sq0 = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; i++)
+        if (t + i * lanes < pieces)
+#pragma unroll
+          for (int j = 0; j < kPiece; j++) {
+            s[i][j] *= kDown;
+            sq0 = fmaf(s[i][j], s[i][j], sq0);
+          }
+      if (!kOneWarp) __syncthreads();   // (the sums of this turn have been read)
+      total = row_sum<kOneWarp>(sq0, sums);
+      inv = inverse_root(total * a.inv_h);
+    }
+    uint8_t *pc = a.codes + row * a.H, *ps = a.scales + row * (a.H / kGroup);
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const int p = t + i * lanes;
+      const bool in = p < pieces;
+      if (in && w) {
+        float wv[kPiece];
         Raw<T> wr;
-        wr.load(w + (size_t)p * kPiece);
+        wr.load(w + p * kPiece);
         wr.get(wv);
-      }
 #pragma unroll
-      for (int j = 0; j < kPiece; j++) s[i][j] = w ? s[i][j] * inv * wv[j] : s[i][j] * inv;
-    }
-    const float amax = group_amax(in ? piece_amax(s[i]) : 0.f);
-    if (in) {
-      const uint32_t byte = scale_byte(amax);
-      *reinterpret_cast<uint2*>(a.codes + row * a.H + (size_t)p * kPiece) = codes_of(s[i], inverse_scale(byte), amax);
-      if ((t & 3) == 0) a.scales[row * (a.H / kGroup) + p / 4] = (uint8_t)byte;
+        for (int j = 0; j < kPiece; j += 2) mul2(s[i][j], s[i][j + 1], s[i][j], s[i][j + 1], wv[j], wv[j + 1]);
+      }
+      const float amax = group_amax(in ? piece_amax(s[i]) : 0.f) * inv;
+      if (in) {
+        const uint32_t byte = scale_byte(amax);
+        float f = inv * inverse_scale(byte);
+        if (byte < 32u) {   // y below 2^-86: inv * 2^-E may leave fp32, so one after the other
+          f = inverse_scale(byte);
+#pragma unroll
+          for (int j = 0; j < kPiece; j++) s[i][j] *= inv;
+        }
+        *reinterpret_cast<uint2*>(pc + p * kPiece) = codes_of(s[i], f, amax);
+        if ((t & 3) == 0) ps[p >> 2] = (uint8_t)byte;
+      }
     }
   }
 }
@@ -219,32 +260,79 @@ struct GateArgs {
 };
 
 constexpr int kGateThreads = 256;
+constexpr int kGatePieces = 2;   // pieces of a thread whose loads are issued together
 
+// g * sigmoid(g) * u for two pairs, through t = exp(-|g|), which does not overflow: g * (g < 0 ? t : 1) / (1 + t) * u.
+// t = 2^(h + l) with h = -|g| * log2(e) rounded and l what the rounding and log2(e)'s own end lose (a product's error is exact in
+// one fused multiplication): 2^h by the hardware, times 1 + l * ln(2).  1 + t is in [1, 2], where a Newton step brings the
+// hardware's reciprocal to the last bit but one.  Under 2^-126 (gates below -87) t is zero.
+UQ_DEV void silu_mul2(float& y0, float& y1, float u0, float u1) {
+  constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596303e-08f, kLn2 = 0.693147181f;   // log2(e) = kLog2e + kLog2eRest
+  const float g0 = y0, g1 = y1, a0 = fmaxf(-fabsf(g0), -200.f), a1 = fmaxf(-fabsf(g1), -200.f);
+  float h0, h1, l0, l1, t0, t1, d0, d1, r0, r1;
+  mul2(h0, h1, a0, a1, kLog2e, kLog2e);
+  fma2(l0, l1, a0, a1, kLog2e, kLog2e, -h0, -h1);
+  fma2(l0, l1, a0, a1, kLog2eRest, kLog2eRest, l0, l1);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(h0));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(h1));
+  mul2(l0, l1, l0, l1, kLn2, kLn2);
+  fma2(t0, t1, t0, t1, l0, l1, t0, t1);
+  add2(d0, d1, t0, t1, 1.f, 1.f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(d0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(d1));
+  fma2(d0, d1, -d0, -d1, r0, r1, 1.f, 1.f);
+  fma2(r0, r1, r0, r1, d0, d1, r0, r1);
+  mul2(y0, y1, g0, g1, g0 < 0.f ? t0 : 1.f, g1 < 0.f ? t1 : 1.f);
+  mul2(y0, y1, y0, y1, r0, r1);
+  mul2(y0, y1, y0, y1, u0, u1);
+}
+
+// The rows' pieces are one sequence, cut into runs of a block's threads: a group's four lanes never leave their row (F is a
+// multiple of 32, runs start at multiples of 4), and no lane is idle for a row's odd end.  A thread's place moves on by
+// (step_row, step_piece), so that nothing is divided on the way.
 template <typename T>
-__global__ void __launch_bounds__(kGateThreads) uq_silu_mul_kernel(GateArgs a, int pdl) {
+__global__ void __launch_bounds__(kGateThreads, 5) uq_silu_mul_kernel(GateArgs a, int pdl) {
   uq_pdl_wait();
   if (pdl) uq_pdl_release();
   const int pieces = a.F / kPiece;
-  for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const int p = blockIdx.x * kGateThreads + threadIdx.x;
-    const bool in = p < pieces;
-    float y[kPiece];
-    if (in) {
-      const T* x = static_cast<const T*>(a.x) + row * 2 * a.F + (size_t)p * kPiece;
-      Raw<T> gr, ur;
-      gr.load(x);
-      ur.load(x + a.F);
-      float g[kPiece], u[kPiece];
-      gr.get(g);
-      ur.get(u);
+  const long long at0 = (long long)blockIdx.x * kGateThreads + threadIdx.x;
+  long long row = at0 / pieces;
+  int p = (int)(at0 - row * pieces);
+  const long long step = (long long)gridDim.x * kGateThreads;
+  const long long step_row = step / pieces;
+  const int step_piece = (int)(step - step_row * pieces);
+  while (__any_sync(0xffffffffu, row < a.rows)) {   // (a warp's lanes leave together: the shuffles need all of them)
+    Raw<T> gr[kGatePieces], ur[kGatePieces];
+    long long at[kGatePieces];
 #pragma unroll
-      for (int j = 0; j < kPiece; j++) y[j] = g[j] / (1.f + expf(-g[j])) * u[j];
+    for (int i = 0; i < kGatePieces; i++) {
+      at[i] = row < a.rows ? row * pieces + p : -1;
+      if (row < a.rows) {
+        const T* x = static_cast<const T*>(a.x) + row * 2 * a.F + (long long)p * kPiece;
+        gr[i].load(x);
+        ur[i].load(x + a.F);
+      }
+      row += step_row;
+      p += step_piece;
+      if (p >= pieces) { p -= pieces; row++; }
     }
-    const float amax = group_amax(in ? piece_amax(y) : 0.f);
-    if (in) {
-      const uint32_t byte = scale_byte(amax);
-      *reinterpret_cast<uint2*>(a.codes + row * a.F + (size_t)p * kPiece) = codes_of(y, inverse_scale(byte), amax);
-      if ((p & 3) == 0) a.scales[row * (a.F / kGroup) + p / 4] = (uint8_t)byte;
+#pragma unroll
+    for (int i = 0; i < kGatePieces; i++) {
+      const bool in = at[i] >= 0;
+      float y[kPiece];
+      if (in) {
+        float u[kPiece];
+        gr[i].get(y);
+        ur[i].get(u);
+#pragma unroll
+        for (int j = 0; j < kPiece; j += 2) silu_mul2(y[j], y[j + 1], u[j], u[j + 1]);
+      }
+      const float amax = group_amax(in ? piece_amax(y) : 0.f);
+      if (in) {
+        const uint32_t byte = scale_byte(amax);
+        *reinterpret_cast<uint2*>(a.codes + at[i] * kPiece) = codes_of(y, inverse_scale(byte), amax);
+        if ((threadIdx.x & 3) == 0) a.scales[at[i] >> 2] = (uint8_t)byte;
+      }
     }
   }
 }
@@ -300,21 +388,44 @@ __global__ void __launch_bounds__(kGateThreads) uq_split_kernel(const __nv_bfloa
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
 
-template <typename T, int V>
-cudaError_t norm_launch(const NormArgs& a, int lanes, cudaStream_t s) {
+// Blocks that the device holds at once (looked up once per kernel and block size, the same on every device of the box).
+template <typename K>
+int resident_blocks(K kern, int threads, int sms, std::atomic<int>* cached) {
+  int n = cached[threads / 32].load(std::memory_order_relaxed);
+  if (!n) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
+    cached[threads / 32].store(n, std::memory_order_relaxed);
+  }
+  return n * sms;
+}
+
+template <typename T, int V, bool kOneWarp>
+cudaError_t norm_launch(const NormArgs& a, cudaStream_t s) {
+  const int pieces = a.H / kPiece, lanes = kOneWarp ? 32 : ((pieces + V - 1) / V + 31) / 32 * 32;
   const bool pdl = uq_pdl_on();
-  if (lanes == 32) return uq_launch(uq_rms_norm_kernel<T, V, true>, dim3((unsigned)((a.rows + 3) / 4)), 128u, 0, s, pdl, a, (int)pdl);
-  return uq_launch(uq_rms_norm_kernel<T, V, false>, dim3((unsigned)a.rows), (unsigned)lanes, 0, s, pdl, a, (int)pdl);
+  return uq_launch(uq_rms_norm_kernel<T, V, kOneWarp>, dim3((unsigned)(kOneWarp ? (a.rows + 3) / 4 : a.rows)), (unsigned)(kOneWarp ? 128 : lanes), 0, s, pdl, a, (int)pdl);
 }
 template <typename T>
 cudaError_t norm_by_size(const NormArgs& a, int sms, cudaStream_t s) {
   const int pieces = a.H / kPiece;
-  (void)sms;
-  const int v = pieces <= 32 ? 1 : (pieces <= 64 ? 2 : 4);
-  const int lanes = ((pieces + v - 1) / v + 31) / 32 * 32;
-  if (v == 1) return norm_launch<T, 1>(a, lanes, s);
-  if (v == 2) return norm_launch<T, 2>(a, lanes, s);
-  return norm_launch<T, 4>(a, lanes, s);
+  if (pieces <= 32) return norm_launch<T, 1, true>(a, s);
+  if (pieces <= 64) return norm_launch<T, 2, true>(a, s);
+  if (pieces <= 128) return norm_launch<T, 4, true>(a, s);
+  // A piece per thread while all rows fit the device at once, four from there on (us with one / four, bf16 with a residual:
+  // 4096 channels, 8 rows 1.76 / 2.62, 296 rows 2.33 / 3.15, 1184 rows 5.90 / 5.04; 8192 channels, 8 rows 2.33 / 2.86, 296 rows 3.69 / 3.81,
+  // 592 rows 6.64 / 4.79).
+  const bool few = a.rows * pieces <= 2048ll * sms;
+  if (pieces <= 1024 && few) return norm_launch<T, 1, false>(a, s);
+  if (pieces <= 2048 && few) return norm_launch<T, 2, false>(a, s);
+  return norm_launch<T, 4, false>(a, s);
+}
+template <typename T>
+cudaError_t gate_launch(const GateArgs& a, int sms, cudaStream_t s) {
+  static std::atomic<int> cached[33];
+  const long long all = a.rows * (a.F / kPiece), want = (all + kGateThreads - 1) / kGateThreads;
+  const long long most = resident_blocks(uq_silu_mul_kernel<T>, kGateThreads, sms, cached);
+  const bool pdl = uq_pdl_on();
+  return uq_launch(uq_silu_mul_kernel<T>, dim3((unsigned)(want < most ? want : most)), (unsigned)kGateThreads, 0, s, pdl, a, (int)pdl);
 }
 
 }  // namespace
@@ -322,11 +433,11 @@ cudaError_t norm_by_size(const NormArgs& a, int sms, cudaStream_t s) {
 // dtype: 0 fp32, 1 bf16, 2 fp16 (of x, r, w and the sum)
 cudaError_t uq_rms_norm_dispatch(const void* x, const void* r, const void* w, void* sum, uint8_t* codes, uint8_t* scales, long long rows, int H, int dtype, float eps,
                                  int sms, cudaStream_t s) {
-  if (rows < 0 || rows > INT_MAX || H < kGroup || H > 32768 || H % kGroup || dtype < 0 || dtype > 2 || !(eps > 0.f)) return cudaErrorInvalidValue;
+  if (rows < 0 || rows > INT_MAX || H < kGroup || H > 32768 || H % kGroup || dtype < 0 || dtype > 2 || !(eps >= 1.17549435e-38f)) return cudaErrorInvalidValue;
   if (rows == 0) return cudaSuccess;
   if (!x || !codes || !scales || (r != nullptr) != (sum != nullptr)) return cudaErrorInvalidValue;
   if (!aligned16(x) || !aligned16(r) || !aligned16(w) || !aligned16(sum) || !aligned8(codes)) return cudaErrorInvalidValue;
-  const NormArgs a{x, r, w, sum, codes, scales, rows, H, eps};
+  const NormArgs a{x, r, w, sum, codes, scales, rows, H, 1.f / (float)H, eps};
   switch (dtype) {
     case 0: return norm_by_size<float>(a, sms, s);
     case 1: return norm_by_size<__nv_bfloat16>(a, sms, s);
@@ -334,17 +445,15 @@ cudaError_t uq_rms_norm_dispatch(const void* x, const void* r, const void* w, vo
   }
 }
 
-cudaError_t uq_silu_mul_dispatch(const void* x, uint8_t* codes, uint8_t* scales, long long rows, int F, int dtype, cudaStream_t s) {
+cudaError_t uq_silu_mul_dispatch(const void* x, uint8_t* codes, uint8_t* scales, long long rows, int F, int dtype, int sms, cudaStream_t s) {
   if (rows < 0 || rows > INT_MAX || F < kGroup || F > (1 << 20) || F % kGroup || dtype < 0 || dtype > 2) return cudaErrorInvalidValue;
   if (rows == 0) return cudaSuccess;
   if (!x || !codes || !scales || !aligned16(x) || !aligned8(codes)) return cudaErrorInvalidValue;
   const GateArgs a{x, codes, scales, rows, F};
-  const bool pdl = uq_pdl_on();
-  const dim3 grid((unsigned)((F / kPiece + kGateThreads - 1) / kGateThreads), (unsigned)(rows < 32768 ? rows : 32768));
   switch (dtype) {
-    case 0: return uq_launch(uq_silu_mul_kernel<float>, grid, (unsigned)kGateThreads, 0, s, pdl, a, (int)pdl);
-    case 1: return uq_launch(uq_silu_mul_kernel<__nv_bfloat16>, grid, (unsigned)kGateThreads, 0, s, pdl, a, (int)pdl);
-    default: return uq_launch(uq_silu_mul_kernel<__half>, grid, (unsigned)kGateThreads, 0, s, pdl, a, (int)pdl);
+    case 0: return gate_launch<float>(a, sms, s);
+    case 1: return gate_launch<__nv_bfloat16>(a, sms, s);
+    default: return gate_launch<__half>(a, sms, s);
   }
 }
 

@@ -501,16 +501,26 @@ def quantize_on_write(x, code, scale, slots, rule="ceil", c=None, kernel=None):
 
 
 # ---- the operators around a layer's attention (not in the reference) -----------------------------------------------
-def _same_device(first, *others):
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError("uq_cuda: tensors must live on one device")
+# Their checks, allocations and launches are in csrc/uq_host.cpp: a decode step calls them several times per layer for 2.5 to 6 us of
+# GPU work each, and the same steps in Python cost the host two to three times that.
+_HOST_FNS = ("uqb_plan_step_launch", "uqb_rms_norm_mx8_launch", "uqb_silu_mul_mx8_launch", "uqb_fp4_linear_scratch_bytes", "uqb_fp4_linear_launch")
+_host_module = None
 
 
-def _rows(t):
-    """Contiguous and 16-byte aligned, as the row kernels read it (a copy where it is not)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _host():
+    """The host module, bound to the loaded library.  Raises if it has not been built (python -m all_quant_b200.build)."""
+    global _host_module
+    if _host_module is None:
+        import importlib.util
+        path = os.path.join(_HERE, "_uq_host.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python -m all_quant_b200.build` (there is no fallback path)")
+        spec = importlib.util.spec_from_file_location("_uq_host", path)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m.bind(*(ctypes.cast(getattr(lib(), f), ctypes.c_void_p).value for f in _HOST_FNS))
+        _host_module = m
+    return _host_module
 
 
 def plan_step(seq_lens, new_tokens, block_table, page_size, num_tokens, *, free_pages=None, slots=None):
@@ -527,52 +537,7 @@ def plan_step(seq_lens, new_tokens, block_table, page_size, num_tokens, *, free_
     append_kv skips) for rows behind the last request's tokens, for positions outside the table, and where no page was left.
     taken int32 [1]: free pages needed (None without free_pages); more than F means that the entries beyond are -1.
     num_tokens bounds the token axis and fixes the shape of slots: a captured graph may be padded.  B <= 16384."""
-    starts, K = (new_tokens, 0) if torch.is_tensor(new_tokens) else (None, int(new_tokens or 0))
-    _need_cuda(seq_lens, starts, block_table, free_pages, slots)
-    _same_device(seq_lens, starts, block_table, free_pages, slots)
-    B = seq_lens.shape[0]
-    if seq_lens.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] < B or block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise RuntimeError("seq_lens [B], block_table int32 [>= B, max_pages] with contiguous rows")
-    if starts is not None and (starts.dim() != 1 or starts.shape[0] != B + 1):
-        raise RuntimeError("new_tokens: an int, the B+1 starts, or None")
-    if starts is None and new_tokens is not None and K < 1:
-        raise RuntimeError("new_tokens: at least one per request (None: whole prompts)")
-    if B > 16384 or page_size < 1 or num_tokens < 0:
-        raise RuntimeError("plan_step: at most 16384 requests, page_size >= 1, num_tokens >= 0")
-    if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
-        seq_lens = seq_lens.to(torch.int32).contiguous()
-    if starts is not None and (starts.dtype != torch.int32 or not starts.is_contiguous()):
-        starts = starts.to(torch.int32).contiguous()
-    if slots is None:
-        slots = torch.empty(num_tokens, dtype=torch.int64, device=seq_lens.device)
-    elif slots.dtype != torch.int64 or slots.shape != (num_tokens,) or not slots.is_contiguous():
-        raise RuntimeError("slots must be contiguous int64 [num_tokens]")
-    taken, n_free = None, 0
-    if free_pages is not None:
-        if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
-            raise RuntimeError("free_pages must be contiguous int32 [F]")
-        taken, n_free = torch.empty(1, dtype=torch.int32, device=seq_lens.device), free_pages.shape[0]
-    stride = block_table.stride(0) if block_table.shape[0] > 1 else max(block_table.stride(0), block_table.shape[1])
-    with _on_device(seq_lens.device):
-        err = lib().uqb_plan_step_launch(seq_lens.data_ptr(), None if starts is None else starts.data_ptr(), K, block_table.data_ptr(), stride,
-                                         free_pages.data_ptr() if n_free else None, n_free, slots.data_ptr(), None if taken is None else taken.data_ptr(), B,
-                                         num_tokens, page_size, block_table.shape[1], _stream(seq_lens))
-    if err:
-        _check(err, "uq_plan_step_launch")
-    return slots, taken
-
-
-def _mx8_out(shape, device, codes, scales):
-    if codes is None:
-        codes = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
-    elif codes.dtype != torch.float8_e4m3fn or codes.shape != shape or not codes.is_contiguous() or codes.device != device:
-        raise RuntimeError("codes must be contiguous float8_e4m3fn of the rows' shape on their device")
-    sshape = shape[:-1] + (shape[-1] // 32,)
-    if scales is None:
-        scales = torch.empty(sshape, dtype=torch.uint8, device=device)
-    elif scales.dtype != torch.uint8 or scales.shape != sshape or not scales.is_contiguous() or scales.device != device:
-        raise RuntimeError("scales must be contiguous uint8 [..., channels / 32] on the rows' device")
-    return codes, scales
+    return (_host_module or _host()).plan_step(seq_lens, new_tokens, block_table, page_size, num_tokens, free_pages, slots)
 
 
 def rms_norm_mx8(x, weight=None, residual=None, *, eps=1e-6, codes=None, scales=None, sum_out=None):
@@ -584,54 +549,14 @@ def rms_norm_mx8(x, weight=None, residual=None, *, eps=1e-6, codes=None, scales=
     nothing added / ones).  Returns (codes float8_e4m3fn [..., H], scales uint8 [..., H/32], s rounded to x's dtype - the next
     residual; None without one).  sum_out may be x or residual itself (in place).  The norm is taken of s in fp32, before it is
     rounded.  Rows holding NaN or infinity give NaN codes."""
-    _need_cuda(x, weight, residual, codes, scales, sum_out)
-    _same_device(x, weight, residual, codes, scales, sum_out)
-    if x.dtype not in _DTYPE or (residual is not None and residual.dtype != x.dtype) or (weight is not None and weight.dtype != x.dtype):
-        raise RuntimeError("x must be fp32, bf16 or fp16; residual and weight of the same type")
-    H = x.shape[-1] if x.dim() else 0
-    if H < 32 or H % 32 or H > 32768:
-        raise RuntimeError("rms_norm_mx8: a multiple of 32 channels, 32 to 32768")
-    if (residual is not None and residual.shape != x.shape) or (weight is not None and weight.shape != (H,)):
-        raise RuntimeError("residual has x's shape, weight [H]")
-    if not eps > 0:
-        raise RuntimeError("eps must be positive")
-    if residual is None:
-        if sum_out is not None:
-            raise RuntimeError("sum_out goes with a residual")
-    elif sum_out is None:
-        sum_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif sum_out.dtype != x.dtype or sum_out.shape != x.shape or not sum_out.is_contiguous() or sum_out.data_ptr() % 16:
-        raise RuntimeError("sum_out must be contiguous, 16-byte aligned, of x's shape and type")
-    codes, scales = _mx8_out(x.shape, x.device, codes, scales)
-    x = _rows(x)
-    r = None if residual is None else _rows(residual)
-    w = None if weight is None else _rows(weight)
-    with _on_device(x.device):
-        err = lib().uqb_rms_norm_mx8_launch(x.data_ptr(), None if r is None else r.data_ptr(), None if w is None else w.data_ptr(),
-                                            None if r is None else sum_out.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel() // H, H, _DTYPE[x.dtype],
-                                            eps, _stream(x))
-    if err:
-        _check(err, "uq_rms_norm_mx8_launch")
-    return codes, scales, sum_out
+    return (_host_module or _host()).rms_norm_mx8(x, weight, residual, eps, codes, scales, sum_out)
 
 
 def silu_mul_mx8(x, *, codes=None, scales=None):
     """The gated activation between the two products of a feed-forward block, with the 8-bit output that the second one takes:
     x [..., 2F] fp32, bf16 or fp16 = gates, then factors; e4m3 codes of g / (1 + exp(-g)) * u.  Returns (codes float8_e4m3fn
     [..., F], scales uint8 [..., F/32]); F a multiple of 32.  Values that are not finite give NaN codes."""
-    _need_cuda(x, codes, scales)
-    if x.dtype not in _DTYPE:
-        raise RuntimeError("x must be fp32, bf16 or fp16")
-    F = x.shape[-1] // 2 if x.dim() else 0
-    if F < 32 or x.shape[-1] % 64 or F > 1 << 20:
-        raise RuntimeError("silu_mul_mx8: twice a multiple of 32 channels, up to 2^21 of them")
-    codes, scales = _mx8_out(x.shape[:-1] + (F,), x.device, codes, scales)
-    x = _rows(x)
-    with _on_device(x.device):
-        err = lib().uqb_silu_mul_mx8_launch(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel() // (2 * F), F, _DTYPE[x.dtype], _stream(x))
-    if err:
-        _check(err, "uq_silu_mul_mx8_launch")
-    return codes, scales
+    return (_host_module or _host()).silu_mul_mx8(x, codes, scales)
 
 
 def pack_fp4_weight(w, *, rule="ceil", c=None):
@@ -648,8 +573,7 @@ def pack_fp4_weight(w, *, rule="ceil", c=None):
     scales = torch.zeros(tiles, ks, 128, 4, dtype=torch.uint8, device=w.device)
     if K % 128:
         w = torch.nn.functional.pad(w, (0, ks * 128 - K))
-    quantize_on_write(w.view(N, ks, 128) if w.is_contiguous() else w.reshape(N, ks, 128), codes, scales,
-                      torch.arange(N, dtype=torch.int64, device=w.device), rule, c)
+    quantize_on_write(w.reshape(N, ks, 128), codes, scales, torch.arange(N, dtype=torch.int64, device=w.device), rule, c)
     return codes, scales
 
 
@@ -666,51 +590,7 @@ def fp4_linear(x, wc, ws, n=None, *, scales=None, out=None, out_dtype=None, work
     bf16 values are taken exactly, save for what lies under 2^-21 of the largest of their 32 channels.  n: output channels
     (default: all rows of the tiles).  out_dtype bf16 (default), fp16 or fp32, or `out` [..., n].  workspace: uint8 scratch of
     fp4_linear_scratch_bytes(rows, K) bytes for bf16 rows (nothing is allocated inside then, out given).  Returns [..., n]."""
-    _need_cuda(x, wc, ws, scales, out, workspace)
-    _same_device(x, wc, ws, scales, out, workspace)
-    K = x.shape[-1] if x.dim() else 0
-    if wc.dim() != 4 or wc.shape[2:] != (128, 64) or wc.dtype != torch.uint8 or not wc.is_contiguous():
-        raise RuntimeError("wc must be contiguous uint8 [ceil(n/128), ceil(K/128), 128, 64]")
-    tiles, ks = wc.shape[:2]
-    if ws.shape != (tiles, ks, 128, 4) or ws.dtype != torch.uint8 or not ws.is_contiguous():
-        raise RuntimeError("ws must be contiguous uint8 [ceil(n/128), ceil(K/128), 128, 4]")
-    n = tiles * 128 if n is None else int(n)
-    if K < 32 or K % 32 or -(-K // 128) != ks or n < 1 or -(-n // 128) != tiles:
-        raise RuntimeError(f"x has {K} channels and y {n}: not those of a weight of {tiles} x {ks} tiles (K a multiple of 32)")
-    if scales is None:
-        if x.dtype != torch.bfloat16:
-            raise RuntimeError("x must be bf16, or float8_e4m3fn with scales")
-    elif x.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8 or scales.shape != x.shape[:-1] + (K // 32,):
-        raise RuntimeError("with scales (uint8 [..., K/32]) x must be float8_e4m3fn [..., K]")
-    if out is None:
-        out = torch.empty(x.shape[:-1] + (n,), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=x.device)
-    elif (out_dtype is not None and out.dtype != out_dtype) or out.shape != x.shape[:-1] + (n,) or not out.is_contiguous():
-        raise RuntimeError("out must be contiguous [..., n]")
-    if out.dtype not in _DTYPE:
-        raise RuntimeError("y is bf16, fp16 or fp32")
-    x = _rows(x)
-    M = x.numel() // K
-    xs = None
-    if scales is None:
-        need = _fp4_scratch(M, K)
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-        elif workspace.dtype != torch.uint8 or workspace.numel() < need or not workspace.is_contiguous():
-            raise RuntimeError("scratch too small")
-    else:
-        xs = _rows(scales)
-    with _on_device(x.device):
-        err = lib().uqb_fp4_linear_launch(x.data_ptr(), None if xs is None else xs.data_ptr(), wc.data_ptr(), ws.data_ptr(), out.data_ptr(),
-                                          workspace.data_ptr() if xs is None else None, M, n, K, _DTYPE[out.dtype], _stream(x))
-    if err:
-        _check(err, "uq_fp4_linear_launch")
-    return out
-
-
-def _fp4_scratch(M, K):
-    """uqb_fp4_linear_scratch_bytes in Python: two planes per tile of 64 rows, or of 8, 16 or 32 that hold all (a test holds the two together)."""
-    rows = min(M, 64)
-    return -(-M // 64) * (16 if rows <= 8 else 32 if rows <= 16 else 64 if rows <= 32 else 128) * (K + K // 32) if M > 0 else 0
+    return (_host_module or _host()).fp4_linear(x, wc, ws, n, scales, out, out_dtype, workspace)
 
 
 def uq_decode_partial(q, kc, ks, vc, vs, block_table, seq_lens, pos_offset=None, *, nsplit=None, sm_scale=None, workspace=None,

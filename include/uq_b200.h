@@ -104,7 +104,7 @@ int uqb_plan_step_launch(const int32_t* seq_lens, const int32_t* starts, int K, 
  * dtype 0 = fp32, 1 = bf16, 2 = fp16 (of x, residual, weight and sum); H (F) a multiple of 32; codes 8-byte aligned, the
  * others 16.
  *   rms_norm:  s = x + residual (NULL: x), codes of s / sqrt(mean(s^2) + eps) * weight (NULL: ones), in fp32 throughout; sum
- *              [rows, H] gets s rounded to dtype (NULL exactly when residual is; may be x or residual itself).  H <= 32768, eps > 0.
+ *              [rows, H] gets s rounded to dtype (NULL exactly when residual is; may be x or residual itself).  H <= 32768, eps >= 2^-126.
  *   silu_mul:  x [rows, 2 F] = gates, then factors: codes of g / (1 + exp(-g)) * u. */
 int uqb_rms_norm_mx8_launch(const void* x, const void* residual, const void* weight, void* sum, uint8_t* codes, uint8_t* scales, long long rows, int H,
                             int dtype, float eps, void* stream);

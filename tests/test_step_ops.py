@@ -149,9 +149,11 @@ def test_linear_refuses(over):
     assert L.uqb_launch_count() == n0
 
 
-def test_scratch_sizes_agree():
-    for M, K in ((1, 32), (8, 4096), (64, 8192), (65, 96), (1000, 32768)):
-        assert uq_cuda.fp4_linear_scratch_bytes(M, K) == uq_cuda._fp4_scratch(M, K)
+def test_scratch_sizes():
+    """Two planes of codes and scales: 8, 16, 32 or 64 rows of each, or tiles of 64."""
+    for M, rows in ((1, 16), (8, 16), (9, 32), (16, 32), (17, 64), (33, 128), (64, 128), (65, 256), (1000, 2048)):
+        for K in (32, 96, 8192):
+            assert uq_cuda.fp4_linear_scratch_bytes(M, K) == rows * (K + K // 32)
     assert uq_cuda.fp4_linear_scratch_bytes(0, 64) == 0 and uq_cuda.fp4_linear_scratch_bytes(4, 40) == 0
 
 
