@@ -18,9 +18,12 @@
 // the layout has those of 4 l .. 4 l + 3: the tensor map therefore brings the rows in the order 4 l + j -> 32 j + l (two
 // dimensions of 32 and 4 rows, the outer one first in memory), and the scale bytes are copied as they lie.
 //
-// One CTA per (128 channels, NB rows, range of K); the ranges of one tile are a cluster, whose CTAs lay their fp32 partial tiles out
-// in shared memory and add each other's up in the order of their ranks, each a share of the rows: one launch, no scratch, the same
-// bits every time.  Two CTAs fit an SM, so that their copies overlap and a grid need not be a multiple of the SMs.
+// One CTA per (128 channels, NB rows, range of K); the ranges of one tile are a cluster, each of whose CTAs adds the fp32 partial tiles
+// of all up for its share of the rows, in the order of the ranks: one launch, no scratch, the same bits every time.  Up to 32 operand
+// rows the partials are pushed: stored straight from registers into the owner's shared memory, counted on its barrier, so that nobody
+// waits for the slowest CTA twice (two cluster barriers around a pull took 1.8 of the 4.1 us of a 4-step CTA).  More rows do not fit
+// beside the ring: each CTA lays its tile out over its own ring and the owners read it between two cluster barriers.
+// Two CTAs fit an SM, so that their copies overlap and a grid need not be a multiple of the SMs.
 #include <climits>
 
 #include <algorithm>
@@ -30,9 +33,13 @@
 
 namespace tc {
 
-constexpr int kThreads = 7 * 32;   // warps 0-3: scales of x, then the epilogue; 4: copies of the weight; 5: instructions; 6: copies of x and of the weight's scales
-constexpr int kWarpW = 4, kWarpMma = 5, kWarpX = 6;
+// warps 0-3: scales of x, then the epilogue; 4: instructions; 5, 6: copies of the weight; 7, 8: copies of x and of the weight's scales.
+// A copy holds its thread for some 300 cycles and a step's scales for as many, about what a step may take on an SM: the steps go
+// round the warps of a role.
+constexpr int kThreads = 9 * 32;
+constexpr int kWarpMma = 4, kWarpW = 5, kWarpX = 7;
 constexpr int kMaxSplit = 8;       // CTAs of a cluster
+constexpr uint32_t kNoTmem = 0xffffffffu;   // no address of tensor memory
 
 struct LinearParams {
   const uint8_t* xs;    // [rows of the x map, K / 32]
@@ -50,14 +57,16 @@ struct LinearParams {
 template <int NB, int PLANES>
 struct LinCfg {
   static constexpr int kRows = NB / PLANES;                  // rows of x per CTA
-  static constexpr int kStages = NB <= 32 ? 5 : (NB == 64 ? 4 : 3);   // what half an SM's shared memory holds
+  static constexpr bool kPush = NB / PLANES <= 16;           // partial tiles are pushed into a buffer of their own
+  static constexpr int kStages = NB == 16 || (NB == 32 && !kPush) ? 5 : (NB <= 64 ? 4 : 3);   // what half an SM's shared memory holds
   static constexpr int kA = 128 * 128, kB = NB * 128, kSf = 512;
   static constexpr int oB = kA, oSfa = oB + kB, oSfb = oSfa + kSf, kStage = oSfb + kSf;
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kPRow = 160;                          // floats of one row of the partial tile, see below
-  static constexpr int kP = kRows * kPRow * 4;
-  static constexpr int kBody = (kRing > kP ? kRing : kP) / 1024 * 1024 + 1024;
-  static constexpr int oBarW = kBody, oBarX = oBarW + 8 * kStages, oBarS = oBarX + 8 * kStages, oBarE = oBarS + 8 * kStages, oBarDone = oBarE + 8 * kStages;
+  static constexpr int kPRow = 512;                          // bytes of one row of a partial tile
+  static constexpr int kP = (kPush ? kRows + kMaxSplit - 1 : kRows) * kPRow;   // (an owner's rows x the ranks: at most that many)
+  static constexpr int oP = kPush ? kRing : 0;
+  static constexpr int kBody = oP + kP > kRing ? oP + kP : kRing;
+  static constexpr int oBarIn = kBody, oBarTmem = oBarIn + 8, oBarW = oBarTmem + 8, oBarX = oBarW + 8 * kStages, oBarS = oBarX + 8 * kStages, oBarE = oBarS + 8 * kStages, oBarDone = oBarE + 8 * kStages;
   static constexpr int oTmem = oBarDone + 8, oAbort = oTmem + 4;
   static constexpr int kSmem = oAbort + 4;
   static constexpr int cSf = NB;                             // first column of the scales: 8 per stage (4 of the weight, 4 of x)
@@ -76,9 +85,15 @@ UQ_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x0, int x1, in
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;"
                ::"r"(dst), "l"(map), "r"(x0), "r"(x1), "r"(x2), "r"(x3), "r"(bar), "l"(pol) : "memory");
 }
+UQ_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+UQ_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 UQ_DEV void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
+}
+// four bytes into a CTA of the cluster, counted on the barrier there
+UQ_DEV void st_async(uint32_t addr, float v, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar) : "memory");
 }
 UQ_DEV uint32_t cluster_addr(uint32_t addr, int rank) {
   uint32_t r;
@@ -142,42 +157,40 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   const size_t block0 = (size_t)tile_n * p.ksteps + k0;   // first 128 x 128 block of this CTA's range
   constexpr int kScaleWarps = (NB + 31) / 32;
 
-  if (tid == 0) {
-    for (int s = 0; s < C::kStages; s++) {
-      mbar_init(bar(C::oBarW, s), 1);
-      mbar_init(bar(C::oBarX, s), 1);
-      mbar_init(bar(C::oBarS, s), kScaleWarps);
-      mbar_init(bar(C::oBarE, s), 1);
-    }
-    mbar_init(bar(C::oBarDone, 0), 1);
-    *abort_flag = 0;
+  const long long m0 = (long long)tile_m * C::kRows;
+  const int rows = (int)min((long long)C::kRows, p.M - m0);   // of this tile
+  const int mine = (rows - rank + split - 1) / split;         // rows rank, rank + split, .. are this CTA's to add up
+
+  if (warp == 0) {   // a barrier per lane
+    constexpr int kBars = 3 + 4 * C::kStages;
+    static_assert(kBars <= 32 && C::oBarX == C::oBarW + 8 * C::kStages && C::oBarDone == C::oBarW + 32 * C::kStages, "barriers lie side by side");
+    if (lane < kBars) mbar_init(sm + C::oBarIn + 8 * lane, lane >= 2 + 2 * C::kStages && lane < 2 + 3 * C::kStages ? kScaleWarps : 1);
     fence_barrier_init();
-    // The first blocks of the weight on their way into L2 while the kernel before this one still runs: a hint that reads nothing -
-    // should that kernel write the weight, the lines in L2 are what it writes.
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.wc + block0 * 8192), "r"(min(nk, C::kStages) * 8192) : "memory");
-  }
-  uq_pdl_wait();   // from here on global memory is read and written
-  if (p.pdl) uq_pdl_release();
-  if (warp == kWarpMma) {   // (after the wait: see the verify kernel)
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm + C::oTmem), "n"(C::kCols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    tc_fence_before();
+    if (lane == 0) {
+      *abort_flag = 0;
+      *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem) = kNoTmem;
+    }
+    __syncwarp();
+    if (C::kPush && split > 1 && lane == 0) mbar_expect_tx(bar(C::oBarIn, 0), (uint32_t)(mine * split * C::kPRow));   // (no rows: complete at once)
+  } else if (warp >= kWarpW && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(warp < kWarpX ? &map_w : &map_x) : "memory");   // (launch arguments, not global memory)
   }
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
+  if (C::kPush && split > 1) cluster_arrive();   // every CTA's barriers stand before the first push
+  uq_pdl_wait();   // from here on global memory is read and written
+  if (p.pdl) uq_pdl_release();
 
-  if (warp == kWarpW || warp == kWarpX) {
-    // ---- copies: one thread each for the weight's codes, and for x with the weight's scales (a copy costs its thread some 300 cycles)
+  if (warp >= kWarpW) {
+    // ---- copies: two threads each for the weight's codes, and for x with the weight's scales
     if (elect_one()) {
-      const bool weights = warp == kWarpW;
+      const bool weights = warp < kWarpX;
       const uint64_t pol = l2_policy();
       uint64_t keep;
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
       const int full = weights ? C::oBarW : C::oBarX;
-      int i = 0;
+      int i = weights ? warp - kWarpW : warp - kWarpX;
       bool ok = true;
-      for (; i < nk; i++) {
+      for (; i < nk; i += 2) {
         const int s = i % C::kStages;
         if (i >= C::kStages && !(ok = wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 40, i))) break;
         const uint32_t st = stage_at(s), b = bar(full, s);
@@ -191,11 +204,23 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         }
       }
       if (!ok)   // gave up: what this thread still has in flight lands before the CTA may end
-        for (int j = max(i - C::kStages, 0); j < i; j++) bounded_wait(bar(full, j % C::kStages), (j / C::kStages) & 1, abort_flag, p.status, 41, j);
+        for (int j = i - 2; j >= 0 && j >= i - C::kStages; j -= 2) bounded_wait(bar(full, j % C::kStages), (j / C::kStages) & 1, abort_flag, p.status, 41, j);
     }
   } else if (warp == kWarpMma) {
+    // (tensor memory is taken after the wait: see the verify kernel)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm + C::oTmem), "n"(C::kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    uint32_t tmem = kNoTmem;   // (the address is written before the allocation returns: the first read has it)
+    for (int i = 0; i < (1 << 20) && tmem == kNoTmem; i++) tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
     if (elect_one()) {
-      bool ok = true;
+      bool ok = tmem != kNoTmem;
+      if (ok) {
+        tc_fence_before();
+        mbar_arrive(bar(C::oBarTmem, 0));
+      } else {
+        *abort_flag = 1;
+        uq_report(p.status, 1u, 49u, 0u);
+      }
       for (int i = 0; i < nk && ok; i++) {
         const int s = i % C::kStages;
         const uint32_t parity = (i / C::kStages) & 1;
@@ -214,11 +239,12 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
       if (ok) tc_commit(bar(C::oBarDone, 0));
     }
   } else {
-    // ---- x's scales: thread r has row r's four bytes of every 128 channels, four loads ahead
-    if (warp < kScaleWarps) {
-      const int groups = p.K / 32;
-      const long long row = (long long)tile_m * NB + tid;
-      const bool have = tid < NB && row < p.xrows;
+    // ---- x's scales: thread r of a group of warps has row r's four bytes of the group's steps, two loads ahead
+    {
+      constexpr int kGroups = 4 / kScaleWarps;
+      const int r = (warp % kScaleWarps) * 32 + lane, groups = p.K / 32;
+      const long long row = (long long)tile_m * NB + r;
+      const bool have = r < NB && row < p.xrows;
       const uint8_t* src = p.xs + row * groups;
       auto load = [&](int i) -> uint32_t {
         uint32_t w = 0x7f7f7f7fu;
@@ -231,34 +257,31 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         }
         return w;
       };
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) w[j] = load(j);
-      bool ok = true;
-      for (int i0 = 0; i0 < nk && ok; i0 += 4) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int i = i0 + j;
-          if (i >= nk || !ok) break;
-          const int s = i % C::kStages;
-          if (i >= C::kStages) ok = __all_sync(0xffffffffu, wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 45, i));
-          if (!ok) break;
-          if (tid < NB) *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfb + lane * 16 + warp * 4) = w[j];
-          w[j] = load(i + 4);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::oBarS, s));
-        }
+      int i = warp / kScaleWarps;
+      uint32_t w0 = load(i), w1 = load(i + kGroups);
+      for (; i < nk; i += kGroups) {
+        const int s = i % C::kStages;
+        if (i >= C::kStages && !__all_sync(0xffffffffu, wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 45, i))) break;
+        if (r < NB) *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfb + lane * 16 + (r >> 5) * 4) = w0;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::oBarS, s));
+        w0 = w1;
+        w1 = load(i + 2 * kGroups);
       }
     }
-    // ---- epilogue, first half: the accumulator's lane 32 j + l is channel 4 l + j of the tile.  A row of the partial tile is four runs
-    // of 32 floats, 40 apart: its writers (a run per warp) and its readers (consecutive channels) both meet every bank once.
-    if (wait(bar(C::oBarDone, 0), 0, 46, nk)) {
-      tc_fence_after();
-      float* part = reinterpret_cast<float*>(smem_lin) + warp * 40 + lane;
+    // ---- epilogue, first half: the accumulator's lane 32 j + l is channel 4 l + j of the tile.  A row of a partial tile is four runs of
+    // 32 floats, one per warp.  Pushed, row t goes to the CTA of rank t % split, place (t / split, this rank).
+    const bool ok = __all_sync(0xffffffffu, wait(bar(C::oBarDone, 0), 0, 46, nk) && wait(bar(C::oBarTmem, 0), 0, 47, nk));
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
+    if (ok) tc_fence_after();
+    if (C::kPush && split > 1) cluster_wait();
+    int owner = 0;
+    uint32_t place = sm + C::oP + rank * C::kPRow + tid * 4;   // (row / split, rank)
 #pragma unroll
-      for (int c = 0; c < C::kRows; c += 8) {
-        uint32_t v[8];
+    for (int c = 0; c < C::kRows; c += 8) {
+      uint32_t v[8];
+      if (ok) {
         tmem_ld8(tmem + ((uint32_t)(warp * 32) << 16) + c, v);
         if (PLANES == 2) {
           uint32_t u[8];
@@ -269,54 +292,75 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         } else {
           tc_wait_ld();
         }
+      } else {   // gave up: the failure shows in the output
 #pragma unroll
-        for (int j = 0; j < 8; j++) part[(c + j) * C::kPRow] = __uint_as_float(v[j]);
+        for (int j = 0; j < 8; j++) v[j] = 0x7fc00000u;
       }
-      tc_fence_before();
+      if (C::kPush && split > 1) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          if (c + j < rows) st_async(cluster_addr(place, owner), __uint_as_float(v[j]), cluster_addr(bar(C::oBarIn, 0), owner));
+          if (++owner == split) {
+            owner = 0;
+            place += split * C::kPRow;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) *reinterpret_cast<float*>(smem_lin + C::oP + (c + j) * C::kPRow + tid * 4) = __uint_as_float(v[j]);
+      }
     }
+    if (ok) tc_fence_before();
   }
-  __syncthreads();
-  if (*abort_flag) {   // (the copies in flight have been waited for) the failure shows in the output
-    for (int i = tid; i < C::kRows * C::kPRow; i += kThreads) reinterpret_cast<float*>(smem_lin)[i] = __int_as_float(0x7fc00000);
+  __syncwarp();
+  bool in = true;
+  if (C::kPush && split > 1) {
+    if (warp >= kWarpMma) cluster_wait();   // (every thread that arrived waits once)
+    in = wait(bar(C::oBarIn, 0), 0, 48, nk);
+  } else {
+    __syncthreads();
+    if (!C::kPush && *abort_flag) {   // (a copy that landed late may have covered what says so)
+      for (int i = tid; i < C::kP / 4; i += kThreads) reinterpret_cast<uint32_t*>(smem_lin)[i] = 0x7fc00000u;
+      __syncthreads();
+    }
+    if (split > 1) cluster_sync();
   }
-  if (split > 1) cluster_sync(); else __syncthreads();
   // ---- second half: this CTA's share of the rows, the partial tiles in the order of the ranks.  A warp per row, four consecutive
   // channels per lane; the loads of all ranks are issued before the first addition.
-  {
-    const int n = tile_n * 128 + 4 * lane;
-    const long long m0 = (long long)tile_m * C::kRows;
-    const int rows = (int)min((long long)C::kRows, p.M - m0);
-    for (int t = rank + warp * split; t < rows; t += (kThreads / 32) * split) {
-      const uint32_t at = sm + (uint32_t)(t * C::kPRow + lane) * 4;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (split == 1) {
+  for (int i = warp; i < mine; i += kThreads / 32) {
+    const int t = rank + i * split, n = tile_n * 128 + 4 * lane;
+    float u[kMaxSplit][4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const float*>(smem_lin + (at - sm) + j * 160);
-      } else {
-        float u[kMaxSplit][4];
+    for (int r = 0; r < kMaxSplit; r++)
+      if (r < split) {
+        if (C::kPush || split == 1) {
+          const uint8_t* at = smem_lin + C::oP + (C::kPush ? i * split + r : t) * C::kPRow + lane * 4;
 #pragma unroll
-        for (int r = 0; r < kMaxSplit; r++)
-          if (r < split) {
-            const uint32_t a = cluster_addr(at, r);
+          for (int j = 0; j < 4; j++) u[r][j] = *reinterpret_cast<const float*>(at + j * 128);
+        } else {
+          const uint32_t at = cluster_addr(sm + C::oP + t * C::kPRow + lane * 4, r);
 #pragma unroll
-            for (int j = 0; j < 4; j++) u[r][j] = ld_cluster(a + j * 160);
-          }
-#pragma unroll
-        for (int r = 0; r < kMaxSplit; r++)
-          if (r < split)
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] += u[r][j];
+          for (int j = 0; j < 4; j++) u[r][j] = ld_cluster(at + j * 128);
+        }
       }
-      const size_t o = (size_t)(m0 + t) * p.N + n;
-      if (p.out_dtype == 0) store4(static_cast<float*>(p.out) + o, v, n, p.N);
-      else if (p.out_dtype == 1) store4(static_cast<__nv_bfloat16*>(p.out) + o, v, n, p.N);
-      else store4(static_cast<__half*>(p.out) + o, v, n, p.N);
-    }
+    float v[4] = {u[0][0], u[0][1], u[0][2], u[0][3]};
+#pragma unroll
+    for (int r = 1; r < kMaxSplit; r++)
+      if (r < split)
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] += u[r][j];
+    if (!in) v[0] = v[1] = v[2] = v[3] = __int_as_float(0x7fc00000);
+    const size_t o = (size_t)(m0 + t) * p.N + n;
+    if (p.out_dtype == 0) store4(static_cast<float*>(p.out) + o, v, n, p.N);
+    else if (p.out_dtype == 1) store4(static_cast<__nv_bfloat16*>(p.out) + o, v, n, p.N);
+    else store4(static_cast<__half*>(p.out) + o, v, n, p.N);
   }
-  if (split > 1) cluster_sync();   // nobody leaves while its partial tile is being read
+  if (!C::kPush && split > 1) cluster_sync();   // nobody leaves while its partial tile is being read
+  else __syncthreads();
   if (warp == kWarpMma) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kCols) : "memory");
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
+    if (tmem != kNoTmem) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kCols) : "memory");
   }
 }
 
@@ -390,6 +434,25 @@ int operand_rows(long long r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ?
 int plane_tile(long long M) { return operand_rows(2 * std::min(M, 64ll)); }
 long long plane_rows(long long M) { return (M + 63) / 64 * plane_tile(M); }
 
+// CTAs along K (the cluster) for so many tiles of so many steps.  Calls follow one another on a stream, each kernel's CTAs set up while
+// the one before still runs: with at most a CTA per SM that costs nothing, with more a CTA has to wait for an SM's half to fall
+// free, about 1.4 us; a step less per CTA gains 0.14 to 0.25 us.  So: the most CTAs that leave the second halves free, or, where that
+// saves a CTA more than ten steps, the most that fit both.  (Not quite all: clusters need their SMs in one part of the chip, and from 7/8
+// on some CTAs wait; clusters of seven and eight from half on.)  us from a graph, tiles x steps, first / second choice:
+//   32 x 32 (4096 x 4096) split 4 / 6  5.05 / 6.06     24 x 64 5 / 8  6.19 / 7.21     48 x 32 2 / 5  7.01 / 6.88
+//   64 x 64 2 / 4  11.5 / 10.5     80 x 64 1 / 3  18.5 / 12.1     112 x 32 1 / 2  11.0 / 10.0     64 x 256 2 / 4  36.3 / 25.9
+//   64 bf16 rows: 32 x 32 4 / 5  10.7 / 12.0     64 x 64 2 / 4  21.4 / 18.6
+//   and past the limits: 48 x 32 6 9.0     40 x 40 3 / 7  6.46 / 9.06     16 x 16 6 / 8  3.14 / 4.51
+int pick_split(long long tiles, int steps, int sms) {
+  const int most = std::min(tc::kMaxSplit, steps);
+  int one = 1, two = 1;
+  for (int s = 2; s <= most; s++) {
+    if (8 * tiles * s <= (s >= 7 ? 4 : 7) * sms) one = s;
+    if (8 * tiles * s <= (s == 2 ? 16 : 14) * sms) two = s;
+  }
+  return two > one && (long long)steps * (two - one) > 10ll * one * two ? two : one;
+}
+
 }  // namespace
 
 cudaError_t uq_split_dispatch(const void*, uint8_t*, uint8_t*, long long, int, int, cudaStream_t);
@@ -438,9 +501,7 @@ cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8
   p.out_dtype = out_dtype;
   p.words = K % 128 == 0 && aligned_to(p.xs, 4);
   p.pdl = uq_pdl_on() ? 1 : 0;
-  // CTAs along K: as many as two per SM hold, each with four steps at least
-  const long long fit = 2ll * sms / std::max(1ll, tiles * mtiles);
-  const int split = (int)std::max(1ll, std::min({(long long)tc::kMaxSplit, fit, ksteps / 4}));
+  const int split = pick_split(tiles * mtiles, (int)ksteps, sms);
   cudaError_t e;
   switch (nb * 2 + planes) {
     case 33: e = tc::linear_launch<16, 1>(p, codes, (int)tiles, split, s); break;

@@ -151,10 +151,11 @@ UQ_DEV float row_sum(float v, float* sums) {
   return t;
 }
 
-UQ_DEV float inverse_root(float v) {   // (v is never subnormal: eps is not)
+UQ_DEV float inverse_root(float v) {   // (v is never subnormal: eps is not); a Newton step takes the hardware's 2 ulp to under one
   float r;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
+  const float e = fmaf(-(v * r), r, 1.f);
+  return v < 3e38f ? fmaf(0.5f * r, e, r) : r;   // (infinity and NaN as they are)
 }
 
 // A row per block, or (kOneWarp) per warp; V pieces per lane, the row stays in registers between its two uses.

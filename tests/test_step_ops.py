@@ -496,3 +496,177 @@ def test_linear_refuses_in_python():
                  lambda: uq_cuda.fp4_linear(x, wc, ws, 200, workspace=torch.zeros(10, dtype=torch.uint8, device="cuda"))):
         with pytest.raises(RuntimeError):
             call()
+
+
+# -------------------------------------------------------------------------------------------- streams, graphs, a whole step
+@gpu
+def test_calls_on_another_stream_and_two_at_once():
+    """Two streams at a time, each with its own inputs: what they give is what the default stream gave."""
+    N, K = 640, 2048
+    wc, ws = _weight(N, K, 1)
+    xs = [_rand((24, K), torch.bfloat16, i) for i in range(2)]
+    rs = [_rand((24, K), torch.bfloat16, 10 + i) for i in range(2)]
+
+    def chain(x, r):
+        codes, scales, s = uq_cuda.rms_norm_mx8(x, None, r)
+        return uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales), uq_cuda.fp4_linear(s, wc, ws, N), *uq_cuda.silu_mul_mx8(torch.cat([s, x], 1))
+    want = [chain(x, r) for x, r in zip(xs, rs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(chain(xs[i], rs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(g, want[i]))
+    assert uq_cuda.last_status()[0] == 0
+
+
+@gpu
+def test_captured_and_replayed():
+    """A step's operators in a CUDA graph, replayed on changed inputs, and two graphs whose calls share the caller's workspace on
+    one stream."""
+    N, K, M = 300, 1056, 9
+    wc, ws = _weight(N, K, 1)
+    x, r = _rand((M, K), torch.bfloat16, 1), _rand((M, K), torch.bfloat16, 2)
+    work = torch.empty(uq_cuda.fp4_linear_scratch_bytes(M, K), dtype=torch.uint8, device="cuda")
+    lens, starts = torch.tensor([40, 17], dtype=torch.int32, device="cuda"), torch.tensor([0, 5, 9], dtype=torch.int32, device="cuda")
+    table, free = torch.full((2, 4), 3, dtype=torch.int32, device="cuda"), torch.arange(20, 30, dtype=torch.int32, device="cuda")
+
+    def step():
+        codes, scales, s = uq_cuda.rms_norm_mx8(x, None, r)
+        return (codes, scales, s, uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales), uq_cuda.fp4_linear(s, wc, ws, N, workspace=work),
+                *uq_cuda.plan_step(lens, starts, table, 16, 12, free_pages=free))
+    step()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step())
+        graphs.append(g)
+    for seed in (5, 6):
+        x.copy_(_rand((M, K), torch.bfloat16, seed))
+        lens.copy_(torch.tensor([33 + seed, 20], dtype=torch.int32))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in o] for o in outs]
+        want = step()
+        for o in got:
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(o, want))
+
+
+@gpu
+def test_the_same_bits_every_time():
+    """Partial tiles are added in the order of their ranks, whichever CTA comes first."""
+    for M, N, K in ((1, 4096, 4096), (33, 1000, 8192), (100, 512, 4096)):
+        wc, ws = _weight(N, K, 3)
+        x = _rand((M, K), torch.bfloat16, 4)
+        want = uq_cuda.fp4_linear(x, wc, ws, N, out_dtype=torch.float32)
+        for _ in range(20):
+            assert torch.equal(uq_cuda.fp4_linear(x, wc, ws, N, out_dtype=torch.float32), want)
+
+
+@gpu
+@pytest.mark.parametrize("rotate,page", [(False, 64), (True, 16)])
+def test_a_layers_step(rotate, page):
+    """One layer of a verify step made of the operators and the attention they stand around: norm -> q, k, v -> slots and pages ->
+    append -> verify -> output projection -> norm -> gate and up -> silu_mul -> down, against the same operators called one at
+    a time on tables and slots worked out on the host; and the layer's output against 64 bits."""
+    B, K, HQ, HKV, D, F = 3, 4, 8, 2, 128, 512
+    H = HQ * D
+    g = torch.Generator(device="cuda").manual_seed(7)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    w_qkv, w_o, w_gu, w_d = (uq_cuda.pack_fp4_weight(rnd(n, k) * k ** -0.5) for n, k in ((H + 2 * HKV * D, H), (H, H), (2 * F, H), (H, F)))
+    lens0 = [37, 5, 130]
+    pages = [-(-(n + K) // page) for n in lens0]
+    held = [-(-n // page) for n in lens0]
+    perm = torch.randperm(sum(pages) + 2, generator=g, device="cuda").to(torch.int32)
+    width = max(pages) + 1
+    bt = torch.full((B, width), 0, dtype=torch.int32, device="cuda")
+    at = 0
+    for b in range(B):
+        bt[b, :held[b]] = perm[at:at + held[b]]
+        at += held[b]
+    free = perm[at:].contiguous()
+    caches = [torch.zeros(len(perm), HKV, page, n, dtype=torch.uint8, device="cuda") for n in (D // 2, D // 32, D // 2, D // 32)]
+    # what is stored already, through the operators as well: whole prompts
+    lens_t = torch.tensor(lens0, dtype=torch.int32, device="cuda")
+    slots0, taken0 = vllm_adapter.plan_step(lens_t, None, bt, page, sum(lens0))
+    assert taken0 is None and (slots0 >= 0).all()
+    vllm_adapter.append_kv(*caches, rnd(sum(lens0), HKV, D).bfloat16(), rnd(sum(lens0), HKV, D).bfloat16(), slots0, rotate_k=rotate)
+    hidden, residual = rnd(B * K, H).bfloat16(), rnd(B * K, H).bfloat16()
+    w1, w2 = (1 + 0.1 * rnd(H)).bfloat16(), (1 + 0.1 * rnd(H)).bfloat16()
+    start = torch.arange(0, B * K + 1, K, dtype=torch.int32, device="cuda")
+    assert vllm_adapter.eligible(hidden.view(-1, HQ, D), start, page) == (True, "ok", K)
+    before = [t.clone() for t in caches]
+
+    # the step, nothing between the calls that waits
+    codes, scales, res = uq_cuda.rms_norm_mx8(hidden, w1, residual)
+    qkv = uq_cuda.fp4_linear(codes, *w_qkv, scales=scales)
+    slots, taken = vllm_adapter.plan_step(lens_t + K, start, bt, page, B * K, free_pages=free)
+    k, v = qkv[:, H:H + HKV * D].reshape(-1, HKV, D), qkv[:, H + HKV * D:].reshape(-1, HKV, D)
+    vllm_adapter.append_kv(*caches, k, v, slots, rotate_k=rotate)
+    att = vllm_adapter.uq_verify_attention(qkv[:, :H].reshape(-1, HQ, D), *caches, bt, lens_t + K, K, rotate_q=rotate)
+    o = uq_cuda.fp4_linear(att.view(-1, H), *w_o)
+    codes2, scales2, res2 = uq_cuda.rms_norm_mx8(o, w2, res)
+    gu = uq_cuda.fp4_linear(codes2, *w_gu, scales=scales2)
+    c3, s3 = uq_cuda.silu_mul_mx8(gu)
+    y = uq_cuda.fp4_linear(c3, *w_d, scales=s3)
+    torch.cuda.synchronize()
+
+    # tables and slots on the host
+    want_bt, nxt, want_slots = bt.cpu().clone(), 0, []
+    assert int(taken) == sum(pages) - sum(held)
+    for b, n in enumerate(lens0):
+        for j in range(held[b], pages[b]):
+            assert want_bt[b, j] == free[nxt]
+            nxt += 1
+        want_slots += [int(want_bt[b, p // page]) * page + p % page for p in range(n, n + K)]
+    assert slots.tolist() == want_slots
+    # every link of the chain from its own inputs, in 64 bits
+    s64 = _f64(hidden) + _f64(residual)
+    check_mx8(codes, scales, s64 / np.sqrt((s64 ** 2).mean(-1, keepdims=True) + 1e-6) * _f64(w1))
+    check_linear(qkv, mx8_values(codes, scales), weight64(*w_qkv, H + 2 * HKV * D, H), torch.bfloat16)
+    ref = [t.clone() for t in before]
+    uq_cuda.append_kv(*ref, k, v, torch.tensor(want_slots, device="cuda"), rotate_k=rotate)
+    assert all(torch.equal(a, b) for a, b in zip(caches, ref))
+    q4 = qkv[:, :H].reshape(B, K, HQ, D)
+    assert torch.equal(att, uq_cuda.uq_decode_cuda(uq_cuda.fwht(q4) if rotate else q4, *ref, want_bt.cuda(), torch.tensor([n + K for n in lens0], device="cuda")).view_as(att))
+    check_linear(o, _f64(att.view(-1, H)), weight64(*w_o, H, H), torch.bfloat16, split=True)
+    s64 = _f64(o) + _f64(res)
+    check_mx8(codes2, scales2, s64 / np.sqrt((s64 ** 2).mean(-1, keepdims=True) + 1e-6) * _f64(w2))
+    check_linear(gu, mx8_values(codes2, scales2), weight64(*w_gu, 2 * F, H), torch.bfloat16)
+    g64, u64 = _f64(gu)[:, :F], _f64(gu)[:, F:]
+    check_mx8(c3, s3, g64 / (1 + np.exp(-g64)) * u64)
+    check_linear(y, mx8_values(c3, s3), weight64(*w_d, H, F), torch.bfloat16)
+    assert uq_cuda.last_status()[0] == 0
+
+
+@gpu
+def test_a_captured_step_follows_growing_requests():
+    """The plan in a graph that is replayed as the requests grow: the lengths are the only input that changes, pages come from the
+    free list's front, which the caller moves on by what was taken (a buffer's content, not its address)."""
+    B, page, width, K = 5, 16, 40, 3
+    table, lens = torch.full((B, width), -7, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+    pool = torch.randperm(B * width, device="cuda").to(torch.int32)
+    free = pool.clone()
+    uq_cuda.plan_step(lens + 1, 1, table.clone(), page, B, free_pages=free)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        lens += K
+        slots, taken = uq_cuda.plan_step(lens, K, table, page, B * K + 2, free_pages=free)
+        free.copy_(free[(torch.arange(len(pool), device="cuda") + taken) % len(pool)])
+    n, used, want = 0, 0, np.full((B, width), -7, np.int32)
+    host = pool.cpu().numpy()
+    for _ in range(30):
+        g.replay()
+        want, want_slots, t = plan64([n + K] * B, [K] * B, want, page, B * K + 2, np.concatenate([host[used:], host[:used]]))
+        n, used = n + K, used + t
+        torch.cuda.synchronize()
+        assert slots.tolist() == want_slots.tolist() and int(taken) == t and (table.cpu().numpy() == want).all()
