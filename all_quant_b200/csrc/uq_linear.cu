@@ -9,7 +9,7 @@
 //
 // What bounds it: reading the weight, N * K * 17 / 32 bytes, up to about 128 rows; so nothing is decoded by threads.  The block-scaled
 // tensor instruction (kind::mxf8f6f4, one UE8M0 scale per 32 elements of K) takes the weight's codes and scale bytes as they are,
-// with the 128 output channels as its M and the rows of x as its N:
+// with the 128 output channels as its M and the rows of x as its N (128 of them and a wide weight: the other way round, below):
 //
 //   y^T[n, m] += W[n, k] * X[m, k]     M = 128 channels, N = NB in {16, 32, 64, 128} rows, K = 32 per instruction
 //
@@ -48,7 +48,7 @@ struct LinearParams {
   void* out;
   unsigned int* status;
   long long M, xrows;
-  int N, K, ksteps, mtiles;
+  int N, K, tiles, ksteps, mtiles;
   int out_dtype;
   int words;            // x's scale bytes of 128 channels are aligned words
   int pdl;
@@ -364,6 +364,207 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   }
 }
 
+// ---------------------------------------------------------------------------------------------- 128 operand rows, wide weights
+// More than 64 operand rows (33 to 64 rows of bf16 a tile, 65 to 128 of 8-bit values) and more tiles than SMs.  With the weight as the
+// instruction's 128 rows a step brings 8.5 KB of weight and 16 KB of x, for one use, and writes and reads 64 KB of shared memory (512
+// cycles of its 128 bytes).  Here x's 128 rows are the instruction's M and 256 channels its N: x comes, and is read, once per 256
+// channels: 48 KB per 128 x 128 block of the weight.  One CTA per SM (the accumulators take half of tensor memory), the result is laid out over
+// the ring at the end.
+//
+//   y[m, n] += X[m, k] * W[n, k]     M = 128 rows, N = 256 channels, K = 32 per instruction
+template <int PLANES>
+struct WideCfg {
+  static constexpr int kRows = 128 / PLANES;
+  static constexpr int kStages = 4;
+  static constexpr int kW = 128 * 128, kX = 128 * 128, kSf = 512;   // bytes of one block of the weight, of x, of one block's scales
+  static constexpr int oX = 2 * kW, oSfw = oX + kX, oSfx = oSfw + 2 * kSf, kStage = (oSfx + kSf + 1023) / 1024 * 1024;
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kPRow = 257 * 4;                             // bytes of a row of the result, one per operand row (odd in words: a lane per row writes it)
+  static constexpr int oBarDone = kRing, oBarTmem = oBarDone + 8, oBarW = oBarTmem + 8, oBarX = oBarW + 8 * kStages, oBarS = oBarX + 8 * kStages, oBarE = oBarS + 8 * kStages;
+  static constexpr int oTmem = oBarE + 8 * kStages, oAbort = oTmem + 4;
+  static constexpr int kSmem = oAbort + 4;
+  static constexpr int cSf = 256, kCols = 512;                      // columns of the scales: 12 per stage (4 of x, 8 of the weight)
+  static_assert(128 * kPRow <= kRing && cSf + 12 * kStages <= kCols && kSmem + 1024 <= 228 * 1024, "fits an SM");
+};
+
+template <int PLANES>
+__global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const __grid_constant__ LinearParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+  using C = WideCfg<PLANES>;
+  extern __shared__ __align__(1024) uint8_t smem_lin[];
+  const uint32_t sm = smem_u32(smem_lin);
+  if (sm & 1023u) {   // never expected; the swizzled layouts below would be wrong
+    uq_pdl_wait();
+    if (threadIdx.x == 0) uq_report(p.status, 2u, sm, 1u);
+    return;
+  }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pair = blockIdx.x / p.mtiles, tile_m = blockIdx.x % p.mtiles, nk = p.ksteps;
+  const long long m0 = (long long)tile_m * C::kRows;
+  const int rows = (int)min((long long)C::kRows, p.M - m0);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_lin + C::oAbort);
+  auto stage_at = [&](int s) { return sm + s * C::kStage; };
+  auto bar = [&](int o, int s) { return sm + o + 8 * s; };
+  auto wait = [&](uint32_t b, uint32_t parity, int id, int k) -> bool {
+    bool r = mbar_test(b, parity);
+    if (!r) r = mbar_try(b, parity);
+    if (!r) r = bounded_wait(b, parity, abort_flag, p.status, id, k);
+    return r;
+  };
+  // first blocks of the pair's two tiles (an odd number of tiles: the last one twice, its second copy is never stored)
+  const size_t block[2] = {(size_t)(2 * pair) * nk, (size_t)min(2 * pair + 1, p.tiles - 1) * nk};
+
+  if (warp == 0) {   // a barrier per lane
+    constexpr int kBars = 2 + 4 * C::kStages;
+    static_assert(kBars <= 32 && C::oBarE == C::oBarDone + 8 * (2 + 3 * C::kStages), "barriers lie side by side");
+    if (lane < kBars) mbar_init(sm + C::oBarDone + 8 * lane, lane < 2 || lane >= 2 + 3 * C::kStages ? 1 : (lane < 2 + 2 * C::kStages ? 2 : 4));
+    fence_barrier_init();
+    if (lane == 0) {
+      *abort_flag = 0;
+      *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem) = kNoTmem;
+    }
+  } else if (warp >= kWarpW && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(warp < kWarpX ? &map_w : &map_x) : "memory");   // (launch arguments, not global memory)
+  }
+  __syncthreads();
+  uq_pdl_wait();   // from here on global memory is read and written
+  if (p.pdl) uq_pdl_release();
+
+  if (warp >= kWarpW) {
+    // ---- copies: a thread each for the two blocks of the weight, for x, and for the weight's scales
+    if (elect_one()) {
+      const int role = warp - kWarpW;
+      const uint64_t pol = l2_policy();
+      uint64_t keep;
+      asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
+      const int full = role < 2 ? C::oBarW : C::oBarX;
+      int i = 0;
+      bool ok = true;
+      for (; i < nk; i++) {
+        const int s = i % C::kStages;
+        if (i >= C::kStages && !(ok = wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 50, i))) break;
+        const uint32_t st = stage_at(s), b = bar(full, s);
+        if (role < 2) {
+          mbar_expect_tx(b, 8192);   // the packed bytes are counted
+          tma_load_4d(st + role * C::kW, &map_w, 0, 0, 0, (int)(block[role] + i), b, pol);
+        } else if (role == 2) {
+          mbar_expect_tx(b, C::kX);
+          tma_load_2d(st + C::oX, &map_x, i * 128, tile_m * 128, b, keep);
+        } else {
+          mbar_expect_tx(b, 2 * C::kSf);
+          bulk_load(st + C::oSfw, p.ws + (block[0] + i) * 512, 512, b, pol);
+          bulk_load(st + C::oSfw + C::kSf, p.ws + (block[1] + i) * 512, 512, b, pol);
+        }
+      }
+      if (!ok)   // gave up: what this thread still has in flight lands before the CTA may end
+        for (int j = i - 1; j >= 0 && j >= i - C::kStages; j--) bounded_wait(bar(full, j % C::kStages), (j / C::kStages) & 1, abort_flag, p.status, 51, j);
+    }
+  } else if (warp == kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm + C::oTmem), "n"(C::kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    uint32_t tmem = kNoTmem;   // (the address is written before the allocation returns: the first read has it)
+    for (int i = 0; i < (1 << 20) && tmem == kNoTmem; i++) tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
+    if (elect_one()) {
+      bool ok = tmem != kNoTmem;
+      if (ok) {
+        tc_fence_before();
+        mbar_arrive(bar(C::oBarTmem, 0));
+      } else {
+        *abort_flag = 1;
+        uq_report(p.status, 1u, 59u, 0u);
+      }
+      for (int i = 0; i < nk && ok; i++) {
+        const int s = i % C::kStages;
+        const uint32_t parity = (i / C::kStages) & 1;
+        ok = wait(bar(C::oBarX, s), parity, 52, i) && wait(bar(C::oBarS, s), parity, 53, i) && wait(bar(C::oBarW, s), parity, 54, i);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t st = stage_at(s), sf = tmem + C::cSf + 12 * s;
+        tmem_copy_sf(sf, sf_desc(st + C::oSfx));
+        tmem_copy_sf(sf + 4, sf_desc(st + C::oSfw));
+        tmem_copy_sf(sf + 8, sf_desc(st + C::oSfw + C::kSf));
+        const uint64_t a = smem_desc(st + C::oX, 16, 1024), b = smem_desc(st, 16, 1024);
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++)
+          mma_bs(tmem, a + (uint64_t)(kb * 2), b + (uint64_t)(kb * 2), instr_desc_bs(128, 256, 0, 5, kb, kb), sf, sf + 4, (i || kb) ? 1u : 0u);
+        tc_commit(bar(C::oBarE, s));
+      }
+      if (ok) tc_commit(bar(C::oBarDone, 0));
+    }
+  } else {
+    // ---- x's scales: thread r has row r's four bytes of every step, two loads ahead
+    {
+      const int groups = p.K / 32;
+      const long long row = (long long)tile_m * 128 + tid;
+      const bool have = row < p.xrows;
+      const uint8_t* src = p.xs + row * groups;
+      auto load = [&](int i) -> uint32_t {
+        uint32_t w = 0x7f7f7f7fu;
+        if (have && i < nk) {
+          const int g = i * 4;
+          if (p.words) return *reinterpret_cast<const uint32_t*>(src + g);
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (g + j < groups) w = (w & ~(0xffu << (8 * j))) | ((uint32_t)src[g + j] << (8 * j));
+        }
+        return w;
+      };
+      uint32_t w0 = load(0), w1 = load(1);
+      for (int i = 0; i < nk; i++) {
+        const int s = i % C::kStages;
+        if (i >= C::kStages && !__all_sync(0xffffffffu, wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 55, i))) break;
+        *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfx + lane * 16 + warp * 4) = w0;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::oBarS, s));
+        w0 = w1;
+        w1 = load(i + 2);
+      }
+    }
+    // ---- epilogue, first half: lane = row of the operand, column = channel (in the order of the tensor map)
+    const bool ok = __all_sync(0xffffffffu, wait(bar(C::oBarDone, 0), 0, 56, nk) && wait(bar(C::oBarTmem, 0), 0, 57, nk));
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem) + ((uint32_t)(warp * 32) << 16);
+    if (ok) {
+      tc_fence_after();
+      float* part = reinterpret_cast<float*>(smem_lin + tid * C::kPRow);
+#pragma unroll 2
+      for (int c = 0; c < 256; c += 32) {
+        uint32_t v[32];
+        tmem_ld16(tmem + c, v);
+        tmem_ld16(tmem + c + 16, v + 16);
+        tc_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j++) part[c + j] = __uint_as_float(v[j]);
+      }
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  if (*abort_flag) {   // gave up (the copies in flight have been waited for): the failure shows in the output
+    for (int i = tid; i < 128 * C::kPRow / 4; i += kThreads) reinterpret_cast<uint32_t*>(smem_lin)[i] = 0x7fc00000u;
+    __syncthreads();
+  }
+  // ---- second half, a warp per row: the planes of a row of bf16 are added
+  for (int t = warp; t < rows; t += kThreads / 32) {
+    const float* at = reinterpret_cast<const float*>(smem_lin + t * C::kPRow) + lane;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = PLANES == 2 ? at[32 * j] + at[32 * j + C::kRows * C::kPRow / 4] : at[32 * j];
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const int n = (2 * pair + b) * 128 + 4 * lane;
+      const size_t o = (size_t)(m0 + t) * p.N + n;
+      if (p.out_dtype == 0) store4(static_cast<float*>(p.out) + o, v + 4 * b, n, p.N);
+      else if (p.out_dtype == 1) store4(static_cast<__nv_bfloat16*>(p.out) + o, v + 4 * b, n, p.N);
+      else store4(static_cast<__half*>(p.out) + o, v + 4 * b, n, p.N);
+    }
+  }
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
+    if (tmem != kNoTmem) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kCols) : "memory");
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- host
 // The weight's codes: 128 codes of a row, rows 4 l + j of a block as (l, j), blocks.
 bool weight_map(CUtensorMap* map, const uint8_t* wc, long long blocks) {
@@ -388,25 +589,22 @@ bool x_map(CUtensorMap* map, const uint8_t* x, long long rows, int K, int nb) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NB, int PLANES>
-cudaError_t linear_launch(const LinearParams& p, const uint8_t* x, int tiles, int split, cudaStream_t s) {
-  using C = LinCfg<NB, PLANES>;
-  auto kern = uq_fp4_linear_kernel<NB, PLANES>;
-  static std::atomic<bool> ready[64];
+template <typename K>
+cudaError_t linear_launch(K kern, int smem, std::atomic<bool>* ready, const LinearParams& p, const uint8_t* x, int nb, long long blocks, int split, cudaStream_t s) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!ready[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (!ready[dev].load(std::memory_order_acquire)) {   // per device: the attribute belongs to the device's copy of the kernel
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) { cudaGetLastError(); return e; }
     ready[dev].store(true, std::memory_order_release);
   }
   CUtensorMap mw, mx;
-  if (!weight_map(&mw, p.wc, (long long)tiles * p.ksteps) || !x_map(&mx, x, p.xrows, p.K, NB)) return cudaErrorInvalidValue;
+  if (!weight_map(&mw, p.wc, (long long)p.tiles * p.ksteps) || !x_map(&mx, x, p.xrows, p.K, nb)) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)tiles * p.mtiles, (unsigned)split);
+  cfg.gridDim = dim3((unsigned)blocks, (unsigned)split);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -420,6 +618,16 @@ cudaError_t linear_launch(const LinearParams& p, const uint8_t* x, int tiles, in
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, mw, mx);
   if (e != cudaSuccess) cudaGetLastError();
   return e;
+}
+template <int NB, int PLANES>
+cudaError_t narrow_launch(const LinearParams& p, const uint8_t* x, int split, cudaStream_t s) {
+  static std::atomic<bool> ready[64];
+  return linear_launch(uq_fp4_linear_kernel<NB, PLANES>, LinCfg<NB, PLANES>::kSmem, ready, p, x, NB, (long long)p.tiles * p.mtiles, split, s);
+}
+template <int PLANES>
+cudaError_t wide_launch(const LinearParams& p, const uint8_t* x, cudaStream_t s) {
+  static std::atomic<bool> ready[64];
+  return linear_launch(uq_fp4_linear_wide_kernel<PLANES>, WideCfg<PLANES>::kSmem, ready, p, x, 128, (long long)(p.tiles + 1) / 2 * p.mtiles, 1, s);
 }
 
 }  // namespace tc
@@ -501,17 +709,22 @@ cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8
   p.out_dtype = out_dtype;
   p.words = K % 128 == 0 && aligned_to(p.xs, 4);
   p.pdl = uq_pdl_on() ? 1 : 0;
+  p.tiles = (int)tiles;
+  // 128 operand rows: 256 channels a CTA where the tiles are more than the SMs (64 bf16 rows, us with 128 / 256 channels: 14336 x 4096
+  // 16.5 / 18.2, 16384 x 8192 24.5 / 31.1, 20000 x 4096 22.9 / 18.6, 28672 x 8192 39.8 / 33.9, 65536 x 8192 83 / 72; 128 8-bit rows,
+  // 65536 x 8192 88 / 71): the narrow kernel can then not split K, and with fewer the wide one leaves SMs without work.
+  const bool wide = nb == 128 && tiles * mtiles > sms;
   const int split = pick_split(tiles * mtiles, (int)ksteps, sms);
   cudaError_t e;
   switch (nb * 2 + planes) {
-    case 33: e = tc::linear_launch<16, 1>(p, codes, (int)tiles, split, s); break;
-    case 34: e = tc::linear_launch<16, 2>(p, codes, (int)tiles, split, s); break;
-    case 65: e = tc::linear_launch<32, 1>(p, codes, (int)tiles, split, s); break;
-    case 66: e = tc::linear_launch<32, 2>(p, codes, (int)tiles, split, s); break;
-    case 129: e = tc::linear_launch<64, 1>(p, codes, (int)tiles, split, s); break;
-    case 130: e = tc::linear_launch<64, 2>(p, codes, (int)tiles, split, s); break;
-    case 257: e = tc::linear_launch<128, 1>(p, codes, (int)tiles, split, s); break;
-    default: e = tc::linear_launch<128, 2>(p, codes, (int)tiles, split, s); break;
+    case 33: e = tc::narrow_launch<16, 1>(p, codes, split, s); break;
+    case 34: e = tc::narrow_launch<16, 2>(p, codes, split, s); break;
+    case 65: e = tc::narrow_launch<32, 1>(p, codes, split, s); break;
+    case 66: e = tc::narrow_launch<32, 2>(p, codes, split, s); break;
+    case 129: e = tc::narrow_launch<64, 1>(p, codes, split, s); break;
+    case 130: e = tc::narrow_launch<64, 2>(p, codes, split, s); break;
+    case 257: e = wide ? tc::wide_launch<1>(p, codes, s) : tc::narrow_launch<128, 1>(p, codes, split, s); break;
+    default: e = wide ? tc::wide_launch<2>(p, codes, s) : tc::narrow_launch<128, 2>(p, codes, split, s); break;
   }
   if (e == cudaSuccess) *launches += 1;
   return e;

@@ -420,7 +420,7 @@ def test_linear_bf16_matches_the_plain_form(M, N, K, out):
 
 
 @gpu
-@pytest.mark.parametrize("M,N,K", [(1, 4096, 8192), (3, 2048, 32768), (40, 20000, 1024), (16, 1024, 16384)])
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 8192), (3, 2048, 32768), (40, 20000, 1024), (16, 1024, 16384), (64, 19100, 416), (128, 20001, 288), (200, 9800, 160)])
 def test_linear_long_and_wide(M, N, K):
     wc, ws = _weight(N, K, 5, torch.bfloat16)
     x = _rand((M, K), torch.bfloat16, 6)
