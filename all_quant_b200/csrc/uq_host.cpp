@@ -227,15 +227,15 @@ PyObject* fp4_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const ll M = x.numel() / K;
   if (!scales) {
     const int64_t need = (int64_t)scratch_fn(M, (int)K);
-    if (!work) work = at::empty({need}, x.options().dtype(at::kByte));
-    else REFUSE(work->scalar_type() != at::kByte || work->numel() < need || !work->is_contiguous(), "scratch too small");
+    if (!work && need) work = at::empty({need}, x.options().dtype(at::kByte));
+    REFUSE(work && (work->scalar_type() != at::kByte || work->numel() < need || !work->is_contiguous()), "scratch too small");
   }
   shape.back() = n;
   if (!out) out = at::empty(shape, x.options().dtype(od));
   else REFUSE(out->scalar_type() != od || out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous(), "out must be contiguous bf16, fp16 or fp32 [..., n]");
   const c10::cuda::CUDAGuard on(place.device);
   done(linear_fn(x.data_ptr(), static_cast<uint8_t*>(ptr(scales)), static_cast<uint8_t*>(wc.data_ptr()), static_cast<uint8_t*>(ws.data_ptr()), out->data_ptr(),
-                 scales ? nullptr : work->data_ptr(), M, (int)n, (int)K, dtype_code(od), stream_of(place)),
+                 scales ? nullptr : ptr(work), M, (int)n, (int)K, dtype_code(od), stream_of(place)),
        "uq_fp4_linear_launch");
   return wrap(out);
   END_HANDLE_TH_ERRORS

@@ -4,8 +4,9 @@
 // The weight is laid out as one stream of the paged cache with 128-token pages at head_dim 128 (codes [tiles, K/128, 128, 64],
 // scales [tiles, K/128, 128, 4]: a tile is 128 output channels, a "head" 128 input channels), so the cache's own encoder writes it
 // and every 128 x 128 block is 8 KB of codes and 512 bytes of scales, both contiguous.
-// Activations are e4m3 codes with one UE8M0 scale per 32 channels; bf16 rows are split into two such planes first (uq_rows.cu),
-// whose products are added.
+// Activations are e4m3 codes with one UE8M0 scale per 32 channels; bf16 rows are split into two such planes, whose products are
+// added: up to 4 rows by the CTAs themselves, on their way into shared memory, more by a kernel of their own first (uq_rows.cu), so
+// that not every tile of the weight does it again.
 //
 // What bounds it: reading the weight, N * K * 17 / 32 bytes, up to about 128 rows; so nothing is decoded by threads.  The block-scaled
 // tensor instruction (kind::mxf8f6f4, one UE8M0 scale per 32 elements of K) takes the weight's codes and scale bytes as they are,
@@ -29,20 +30,25 @@
 #include <algorithm>
 #include <atomic>
 
+#include "uq_mx8.cuh"
 #include "uq_sm100.cuh"
 
 namespace tc {
 
-// warps 0-3: scales of x, then the epilogue; 4: instructions; 5, 6: copies of the weight; 7, 8: copies of x and of the weight's scales.
+// warps 0-3: scales of x (or x itself, split), then the epilogue; 4: instructions; 5, 6: copies of the weight; 7, 8: copies of x and of the weight's scales.
 // A copy holds its thread for some 300 cycles and a step's scales for as many, about what a step may take on an SM: the steps go
 // round the warps of a role.
 constexpr int kThreads = 9 * 32;
 constexpr int kWarpMma = 4, kWarpW = 5, kWarpX = 7;
 constexpr int kMaxSplit = 8;       // CTAs of a cluster
+// Rows of bf16 that every CTA splits for itself, without the kernel that does it first (us with it / split in the CTAs: 4096 x 4096 1 row 6.55 / 5.05,
+// 4 rows 6.76 / 5.12, 8 rows 6.83 / 6.35; 28672 x 8192 1 row 25.1 / 23.9, 4 rows 25.2 / 24.6, 6 rows 25.1 / 28.3, 8 rows 25.2 / 33.1).
+constexpr int kDirectRows = 4;
 constexpr uint32_t kNoTmem = 0xffffffffu;   // no address of tensor memory
 
 struct LinearParams {
   const uint8_t* xs;    // [rows of the x map, K / 32]
+  const __nv_bfloat16* x16;   // [M, K] rows that the CTAs split themselves
   const uint8_t* wc;
   const uint8_t* ws;
   void* out;
@@ -131,7 +137,7 @@ UQ_DEV void store4(T* o, const float* v, int n, int N) {
   }
 }
 
-template <int NB, int PLANES>
+template <int NB, int PLANES, bool kDirect>
 __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid_constant__ LinearParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
   using C = LinCfg<NB, PLANES>;
   extern __shared__ __align__(1024) uint8_t smem_lin[];
@@ -198,8 +204,8 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
           mbar_expect_tx(b, 8192);   // the packed bytes are counted
           tma_load_4d(st, &map_w, 0, 0, 0, (int)(block0 + i), b, pol);
         } else {
-          mbar_expect_tx(b, C::kB + C::kSf);
-          tma_load_2d(st + C::oB, &map_x, (k0 + i) * 128, tile_m * NB, b, keep);
+          mbar_expect_tx(b, (kDirect ? 0 : C::kB) + C::kSf);
+          if (!kDirect) tma_load_2d(st + C::oB, &map_x, (k0 + i) * 128, tile_m * NB, b, keep);
           bulk_load(st + C::oSfa, p.ws + (block0 + i) * 512, 512, b, pol);
         }
       }
@@ -239,8 +245,54 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
       if (ok) tc_commit(bar(C::oBarDone, 0));
     }
   } else {
-    // ---- x's scales: thread r of a group of warps has row r's four bytes of the group's steps, two loads ahead
-    {
+    if constexpr (kDirect) {
+      // ---- x itself: a warp splits a step's 4 rows x 128 channels (lane: piece lane % 16 of rows lane / 16 and 2 + lane / 16) into the two planes of the
+      // tile, rows r and 8 + r of 128 bytes with the 128-byte swizzle, and their scale bytes; the next step's loads are on their way.
+      static_assert(!kDirect || (NB == 16 && PLANES == 2), "rows of both planes");
+      constexpr int kPer = kDirectRows / 2;   // pieces of a lane
+      const int piece = lane & 15, r0 = lane >> 4;
+      mx8::Raw<__nv_bfloat16> next[kPer];
+      auto load = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+          const int k = (k0 + i) * 128 + piece * 8;
+          if (2 * j >= rows) break;   // (the tile's rows behind the last one are never written, their products never read)
+          if (i < nk && 2 * j + r0 < rows && k < p.K) next[j].load(p.x16 + (m0 + 2 * j + r0) * p.K + k);
+          else next[j].a = make_uint4(0, 0, 0, 0);
+        }
+      };
+      load(warp);
+      for (int i = warp; i < nk; i += 4) {
+        const int s = i % C::kStages;
+        uint2 hi[kPer], lo[kPer];
+        uint32_t hi_byte[kPer], lo_byte[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+          if (2 * j >= rows) break;
+          float v[8];
+          next[j].get(v);
+          mx8::split_piece(v, hi[j], lo[j], hi_byte[j], lo_byte[j]);
+        }
+        load(i + 4);
+        if (i >= C::kStages && !__all_sync(0xffffffffu, wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 45, i))) break;
+        uint8_t *tile = smem_lin + s * C::kStage + C::oB, *sf = smem_lin + s * C::kStage + C::oSfb + (piece >> 2);
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+          if (2 * j >= rows) break;
+          const int r = 2 * j + r0, at = (((piece >> 1) ^ r) << 4) + (piece & 1) * 8;   // (r < 8: rows r and 8 + r have the same swizzle)
+          *reinterpret_cast<uint2*>(tile + r * 128 + at) = hi[j];
+          *reinterpret_cast<uint2*>(tile + (8 + r) * 128 + at) = lo[j];
+          if ((piece & 3) == 0) {
+            sf[r * 16] = (uint8_t)hi_byte[j];
+            sf[(8 + r) * 16] = (uint8_t)lo_byte[j];
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::oBarS, s));
+      }
+    } else {
+      // ---- x's scales: thread r of a group of warps has row r's four bytes of the group's steps, two loads ahead
       constexpr int kGroups = 4 / kScaleWarps;
       const int r = (warp % kScaleWarps) * 32 + lane, groups = p.K / 32;
       const long long row = (long long)tile_m * NB + r;
@@ -600,7 +652,9 @@ cudaError_t linear_launch(K kern, int smem, std::atomic<bool>* ready, const Line
     ready[dev].store(true, std::memory_order_release);
   }
   CUtensorMap mw, mx;
-  if (!weight_map(&mw, p.wc, (long long)p.tiles * p.ksteps) || !x_map(&mx, x, p.xrows, p.K, nb)) return cudaErrorInvalidValue;
+  if (!weight_map(&mw, p.wc, (long long)p.tiles * p.ksteps)) return cudaErrorInvalidValue;
+  if (!x) mx = mw;   // (not used)
+  else if (!x_map(&mx, x, p.xrows, p.K, nb)) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks, (unsigned)split);
   cfg.blockDim = dim3(kThreads);
@@ -619,10 +673,10 @@ cudaError_t linear_launch(K kern, int smem, std::atomic<bool>* ready, const Line
   if (e != cudaSuccess) cudaGetLastError();
   return e;
 }
-template <int NB, int PLANES>
+template <int NB, int PLANES, bool kDirect = false>
 cudaError_t narrow_launch(const LinearParams& p, const uint8_t* x, int split, cudaStream_t s) {
   static std::atomic<bool> ready[64];
-  return linear_launch(uq_fp4_linear_kernel<NB, PLANES>, LinCfg<NB, PLANES>::kSmem, ready, p, x, NB, (long long)p.tiles * p.mtiles, split, s);
+  return linear_launch(uq_fp4_linear_kernel<NB, PLANES, kDirect>, LinCfg<NB, PLANES>::kSmem, ready, p, x, NB, (long long)p.tiles * p.mtiles, split, s);
 }
 template <int PLANES>
 cudaError_t wide_launch(const LinearParams& p, const uint8_t* x, cudaStream_t s) {
@@ -665,8 +719,8 @@ int pick_split(long long tiles, int steps, int sms) {
 
 cudaError_t uq_split_dispatch(const void*, uint8_t*, uint8_t*, long long, int, int, cudaStream_t);
 
-// Bytes of scratch for bf16 activations: both planes' codes, then their scales.
-size_t uq_fp4_linear_scratch(long long M, int K) { return M < 1 || K < 32 || K % 32 ? 0 : (size_t)plane_rows(M) * ((size_t)K + K / 32); }
+// Bytes of scratch for bf16 activations: both planes' codes, then their scales (none for rows that the CTAs split themselves).
+size_t uq_fp4_linear_scratch(long long M, int K) { return M <= tc::kDirectRows || K < 32 || K % 32 ? 0 : (size_t)plane_rows(M) * ((size_t)K + K / 32); }
 
 // xs null: x is bf16 [M, K], scratch holds uq_fp4_linear_scratch bytes; else x is e4m3 [M, K] with scale bytes xs [M, K / 32].
 // launches: kernels enqueued.
@@ -675,8 +729,9 @@ cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8
   *launches = 0;
   if (M < 0 || M > (1 << 24) || N < 1 || N > (1 << 24) || K < 32 || K > (1 << 24) || K % 32 || out_dtype < 0 || out_dtype > 2) return cudaErrorInvalidValue;
   if (M == 0) return cudaSuccess;
-  if (!x || !wc || !ws || !out || (!xs && !scratch)) return cudaErrorInvalidValue;
-  if (!aligned_to(x, 16) || !aligned_to(wc, 32) || !aligned_to(ws, 16) || !aligned_to(out, 16) || (xs ? !aligned_to(xs, 4) : !aligned_to(scratch, 16))) return cudaErrorInvalidValue;
+  const bool direct = !xs && M <= tc::kDirectRows;
+  if (!x || !wc || !ws || !out || (!xs && !direct && !scratch)) return cudaErrorInvalidValue;
+  if (!aligned_to(x, 16) || !aligned_to(wc, 32) || !aligned_to(ws, 16) || !aligned_to(out, 16) || (xs ? !aligned_to(xs, 4) : !direct && !aligned_to(scratch, 16))) return cudaErrorInvalidValue;
   const long long tiles = (N + 127) / 128, ksteps = (K + 127) / 128;
   const int planes = xs ? 1 : 2;
   const int nb = planes == 2 ? plane_tile(M) : operand_rows(M);
@@ -687,7 +742,10 @@ cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8
   const uint8_t* codes = static_cast<const uint8_t*>(x);
   p.xs = xs;
   p.xrows = M;
-  if (planes == 2) {
+  if (direct) {
+    p.x16 = static_cast<const __nv_bfloat16*>(x);
+    codes = nullptr;
+  } else if (planes == 2) {
     p.xrows = plane_rows(M);
     uint8_t* c = static_cast<uint8_t*>(scratch);
     uint8_t* sc = c + (size_t)p.xrows * K;
@@ -718,7 +776,7 @@ cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8
   cudaError_t e;
   switch (nb * 2 + planes) {
     case 33: e = tc::narrow_launch<16, 1>(p, codes, split, s); break;
-    case 34: e = tc::narrow_launch<16, 2>(p, codes, split, s); break;
+    case 34: e = direct ? tc::narrow_launch<16, 2, true>(p, codes, split, s) : tc::narrow_launch<16, 2>(p, codes, split, s); break;
     case 65: e = tc::narrow_launch<32, 1>(p, codes, split, s); break;
     case 66: e = tc::narrow_launch<32, 2>(p, codes, split, s); break;
     case 129: e = tc::narrow_launch<64, 1>(p, codes, split, s); break;

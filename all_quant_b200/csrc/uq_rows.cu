@@ -16,114 +16,11 @@
 #include <atomic>
 #include <climits>
 
-#include "uq_common.cuh"
+#include "uq_mx8.cuh"
 
 namespace {
 
-constexpr int kPiece = 8;     // channels of a lane's load
-constexpr int kGroup = 32;    // channels of a scale
-
-// ---- pieces: 8 channels of a row as fp32 ----------------------------------------------------------------------------
-template <typename T> struct Raw;
-template <> struct Raw<float> {
-  float4 a, b;
-  UQ_DEV void load(const float* p) { a = *reinterpret_cast<const float4*>(p); b = *reinterpret_cast<const float4*>(p + 4); }
-  UQ_DEV void get(float* v) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w; }
-  UQ_DEV static void store(float* p, const float* v) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  }
-};
-template <> struct Raw<__nv_bfloat16> {
-  uint4 a;
-  UQ_DEV void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
-  UQ_DEV void get(float* v) const {
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
-  UQ_DEV static void store(__nv_bfloat16* p, const float* v) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-template <> struct Raw<__half> {
-  uint4 a;
-  UQ_DEV void load(const __half* p) { a = *reinterpret_cast<const uint4*>(p); }
-  UQ_DEV void get(float* v) const {
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
-  UQ_DEV static void store(__half* p, const float* v) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-
-// ---- the quantiser --------------------------------------------------------------------------------------------------
-// Two operations per issue slot: these kernels run out of those first.
-UQ_DEV void mul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
-      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-UQ_DEV void add2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}"
-      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-UQ_DEV void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {   // d = a * b + c
-  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
-      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
-}
-UQ_DEV float max3(float a, float b, float c) {   // (a NaN is left out: its own code says it)
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-UQ_DEV float piece_amax(const float* v) {
-  const float a = max3(fabsf(v[0]), fabsf(v[1]), fabsf(v[2])), b = max3(fabsf(v[3]), fabsf(v[4]), fabsf(v[5]));
-  return fmaxf(max3(a, fabsf(v[6]), fabsf(v[7])), b);
-}
-UQ_DEV float group_amax(float m) {   // over the four lanes of a group
-  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  return fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-}
-// The scale byte E + 127 for a group's largest magnitude.  448 = 1.75 * 2^8: E = (exponent of amax) - 8, one more where its
-// mantissa is above 1.75; -127 at the lower end (zero and amax below 448 * 2^-127), 121 at most.
-UQ_DEV uint32_t scale_byte(float amax) {
-  const uint32_t b = __float_as_uint(amax);
-  return (uint32_t)max((int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0), 0);
-}
-// 2^-E of such a byte, byte <= 248: exponent field 254 - byte
-UQ_DEV float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
-UQ_DEV uint32_t e4m3x2(float lo, float hi) {
-  unsigned short d;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-// Codes of a piece: e4m3(v * inv), NaN where `amax`, its group's, says that there is an infinity and it is this value (the
-// conversion would saturate it).
-UQ_DEV uint2 codes_of(const float* v, float inv, float amax) {
-  float q[kPiece];
-#pragma unroll
-  for (int i = 0; i < kPiece; i += 2) mul2(q[i], q[i + 1], v[i], v[i + 1], inv, inv);
-  if (__float_as_uint(amax) >= 0x7f800000u) {
-#pragma unroll
-    for (int i = 0; i < kPiece; i++) q[i] = fabsf(v[i]) <= 3.4028235e38f ? q[i] : __int_as_float(0x7fc00000);
-  }
-  return make_uint2(e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16), e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16));
-}
+using namespace mx8;
 
 // ---- norm -----------------------------------------------------------------------------------------------------------
 struct NormArgs {
@@ -341,12 +238,6 @@ __global__ void __launch_bounds__(kGateThreads, 5) uq_silu_mul_kernel(GateArgs a
 // ---- split of bf16 rows into two planes -------------------------------------------------------------------------------
 // Rows are laid out as uq_linear.cu reads them: tiles of tile_rows rows, a tile's leading planes, then its remainder planes; what
 // fills up the last tile is never written, its products never read.
-UQ_DEV void e4m3x2_to_f32(uint32_t v, float& lo, float& hi) {
-  uint32_t h2;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((unsigned short)v));
-  lo = __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu)));
-  hi = __half2float(__ushort_as_half((unsigned short)(h2 >> 16)));
-}
 __global__ void __launch_bounds__(kGateThreads) uq_split_kernel(const __nv_bfloat16* x, uint8_t* codes, uint8_t* scales, long long rows, int K, int tile_rows, int pdl) {
   uq_pdl_wait();
   if (pdl) uq_pdl_release();
@@ -356,32 +247,23 @@ __global__ void __launch_bounds__(kGateThreads) uq_split_kernel(const __nv_bfloa
   for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
     const long long hi_row = row + row / tile_rows * tile_rows, lo_row = hi_row + tile_rows;
     float v[kPiece];
+#pragma unroll
+    for (int j = 0; j < kPiece; j++) v[j] = 0.f;
     if (in) {
       Raw<__nv_bfloat16> xr;
       xr.load(x + row * K + (size_t)p * kPiece);
       xr.get(v);
     }
-    float amax = group_amax(in ? piece_amax(v) : 0.f);
-    uint32_t byte = scale_byte(amax);
-    const uint2 hi = in ? codes_of(v, inverse_scale(byte), amax) : make_uint2(0, 0);
+    uint2 hi, lo;
+    uint32_t hi_byte, lo_byte;
+    split_piece(v, hi, lo, hi_byte, lo_byte);
     if (in) {
       *reinterpret_cast<uint2*>(codes + hi_row * K + (size_t)p * kPiece) = hi;
-      if ((p & 3) == 0) scales[hi_row * (K / kGroup) + p / 4] = (uint8_t)byte;
-      const float scale = uq_scale_f32(byte);
-      const uint32_t h[4] = {hi.x & 0xffffu, hi.x >> 16, hi.y & 0xffffu, hi.y >> 16};
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float a, b;
-        e4m3x2_to_f32(h[i], a, b);
-        v[2 * i] = fmaf(-a, scale, v[2 * i]);           // exact: both are multiples of x's last bit, at most 8 bits apart
-        v[2 * i + 1] = fmaf(-b, scale, v[2 * i + 1]);
+      *reinterpret_cast<uint2*>(codes + lo_row * K + (size_t)p * kPiece) = lo;
+      if ((p & 3) == 0) {
+        scales[hi_row * (K / kGroup) + p / 4] = (uint8_t)hi_byte;
+        scales[lo_row * (K / kGroup) + p / 4] = (uint8_t)lo_byte;
       }
-    }
-    amax = group_amax(in ? piece_amax(v) : 0.f);
-    byte = scale_byte(amax);
-    if (in) {
-      *reinterpret_cast<uint2*>(codes + lo_row * K + (size_t)p * kPiece) = codes_of(v, inverse_scale(byte), amax);
-      if ((p & 3) == 0) scales[lo_row * (K / kGroup) + p / 4] = (uint8_t)byte;
     }
   }
 }

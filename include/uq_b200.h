@@ -116,7 +116,7 @@ int uqb_silu_mul_mx8_launch(const void* x, uint8_t* codes, uint8_t* scales, long
  *               128 h.. are head h.  uqb_append_ex_launch writes it (key = the weight as [N, K/128, 128], slots 0..N-1);
  *               channels behind K and rows behind N have finite scales (the append leaves zero codes there when they are zero).
  *   x, xs       xs NULL: x is bf16 [M, K], taken as two e4m3 planes (exact but for what lies under 2^-21 of a group's largest),
- *               scratch holds uqb_fp4_linear_scratch_bytes(M, K) bytes; else x e4m3 [M, K], xs its scale bytes [M, K/32].
+ *               scratch holds uqb_fp4_linear_scratch_bytes(M, K) bytes (none up to 4 rows: may be NULL); else x e4m3 [M, K], xs its scale bytes [M, K/32].
  *   out         [M, N], out_dtype 0 = fp32, 1 = bf16, 2 = fp16.
  * K a multiple of 32, wc 32-byte aligned, x / ws / out / scratch 16, xs 4.  A row of x that holds NaN or infinity (bf16), or a
  * NaN code, gives NaN in its outputs; other rows are not touched by it. */

@@ -141,7 +141,7 @@ def test_silu_refuses(over):
                                   dict(x=_p(0, 8)), dict(wc=_p(2, 16)), dict(ws=_p(3, 8)), dict(out=_p(4, 8)), dict(xs=_p(1, 2)), dict(xs=None, scratch=None),
                                   dict(xs=None, scratch=_p(5, 8))])
 def test_linear_refuses(over):
-    a = dict(x=_p(0), xs=_p(1), wc=_p(2), ws=_p(3), out=_p(4), scratch=_p(5), M=4, N=128, K=64, dtype=1)
+    a = dict(x=_p(0), xs=_p(1), wc=_p(2), ws=_p(3), out=_p(4), scratch=_p(5), M=9, N=128, K=64, dtype=1)
     a.update(over)
     L = uq_cuda.lib()
     n0 = L.uqb_launch_count()
@@ -150,8 +150,8 @@ def test_linear_refuses(over):
 
 
 def test_scratch_sizes():
-    """Two planes of codes and scales: 8, 16, 32 or 64 rows of each, or tiles of 64."""
-    for M, rows in ((1, 16), (8, 16), (9, 32), (16, 32), (17, 64), (33, 128), (64, 128), (65, 256), (1000, 2048)):
+    """Both planes of codes and scales: 16, 32, 64 or 128 rows, or tiles of 128; none up to 4 rows."""
+    for M, rows in ((1, 0), (4, 0), (5, 16), (8, 16), (9, 32), (16, 32), (17, 64), (33, 128), (64, 128), (65, 256), (1000, 2048)):
         for K in (32, 96, 8192):
             assert uq_cuda.fp4_linear_scratch_bytes(M, K) == rows * (K + K // 32)
     assert uq_cuda.fp4_linear_scratch_bytes(0, 64) == 0 and uq_cuda.fp4_linear_scratch_bytes(4, 40) == 0
@@ -395,7 +395,7 @@ def test_pack_is_the_caches_encoder(N, K, rule):
     assert (wc.transpose(1, 2).reshape(-1, wc.shape[1] * 64)[N:] == 0).all()
 
 
-SHAPES = [(1, 128, 128), (1, 1, 32), (2, 130, 160), (8, 256, 1024), (5, 1000, 1120), (17, 640, 4096), (33, 257, 96), (64, 384, 2048), (65, 129, 288), (127, 512, 256), (128, 300, 512), (130, 256, 640), (300, 128, 224)]
+SHAPES = [(1, 128, 128), (1, 1, 32), (2, 130, 160), (3, 77, 736), (4, 500, 2048), (8, 256, 1024), (5, 1000, 1120), (17, 640, 4096), (33, 257, 96), (64, 384, 2048), (65, 129, 288), (127, 512, 256), (128, 300, 512), (130, 256, 640), (300, 128, 224)]
 
 
 @gpu
@@ -450,17 +450,18 @@ def test_linear_every_code_and_scale():
 
 
 @gpu
-def test_linear_rows_do_not_touch_each_other_and_nothing_beyond_is_written():
+@pytest.mark.parametrize("M", [7, 20, 40])
+def test_linear_rows_do_not_touch_each_other_and_nothing_beyond_is_written(M):
     N, K = 200, 288
     wc, ws = _weight(N, K, 9)
-    x = _rand((20, K), torch.bfloat16, 9)
+    x = _rand((M, K), torch.bfloat16, 9)
     want = uq_cuda.fp4_linear(x, wc, ws, N)
-    x[3, 7], x[11, 280], x[19, 0] = float("nan"), float("inf"), float("-inf")
-    buf = torch.full((24, N), 5.0, dtype=torch.bfloat16, device="cuda")
-    got = uq_cuda.fp4_linear(x, wc, ws, N, out=buf[2:22])   # (2 * 200 * 2 bytes: on its 16-byte boundary)
-    bad = torch.zeros(20, dtype=torch.bool, device="cuda")
-    bad[[3, 11, 19]] = True
-    assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad]) and (buf[:2] == 5).all() and (buf[22:] == 5).all()
+    x[3, 7], x[5, 280], x[M - 1, 0] = float("nan"), float("inf"), float("-inf")
+    buf = torch.full((M + 4, N), 5.0, dtype=torch.bfloat16, device="cuda")
+    got = uq_cuda.fp4_linear(x, wc, ws, N, out=buf[2:M + 2])   # (2 * 200 * 2 bytes: on its 16-byte boundary)
+    bad = torch.zeros(M, dtype=torch.bool, device="cuda")
+    bad[[3, 5, M - 1]] = True
+    assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad]) and (buf[:2] == 5).all() and (buf[M + 2:] == 5).all()
     codes, scales, _ = uq_cuda.rms_norm_mx8(x)
     assert uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales)[3].isnan().all()
     # zero rows and zero values
@@ -493,7 +494,8 @@ def test_linear_refuses_in_python():
     for call in (lambda: uq_cuda.fp4_linear(x.half(), wc, ws), lambda: uq_cuda.fp4_linear(x[:, :256], wc, ws), lambda: uq_cuda.fp4_linear(x, wc, ws, 300), lambda: uq_cuda.fp4_linear(x, wc, ws, 128),
                  lambda: uq_cuda.fp4_linear(x, wc, ws[:, :2].contiguous()), lambda: uq_cuda.fp4_linear(x, wc, ws, scales=torch.zeros(4, 9, dtype=torch.uint8, device="cuda")),
                  lambda: uq_cuda.fp4_linear(x, wc, ws, 200, out=torch.zeros(4, 256, device="cuda")), lambda: uq_cuda.fp4_linear(x, wc, ws, out_dtype=torch.float64),
-                 lambda: uq_cuda.fp4_linear(x, wc, ws, 200, workspace=torch.zeros(10, dtype=torch.uint8, device="cuda"))):
+                 lambda: uq_cuda.fp4_linear(x, wc, ws, 200, workspace=torch.zeros(10, device="cuda")),
+                 lambda: uq_cuda.fp4_linear(x.repeat(3, 1), wc, ws, 200, workspace=torch.zeros(3000, dtype=torch.uint8, device="cuda"))):
         with pytest.raises(RuntimeError):
             call()
 
@@ -529,7 +531,7 @@ def test_calls_on_another_stream_and_two_at_once():
 def test_captured_and_replayed():
     """A step's operators in a CUDA graph, replayed on changed inputs, and two graphs whose calls share the caller's workspace on
     one stream."""
-    N, K, M = 300, 1056, 9
+    N, K, M = 300, 1056, 9   # (nine bf16 rows: with the workspace)
     wc, ws = _weight(N, K, 1)
     x, r = _rand((M, K), torch.bfloat16, 1), _rand((M, K), torch.bfloat16, 2)
     work = torch.empty(uq_cuda.fp4_linear_scratch_bytes(M, K), dtype=torch.uint8, device="cuda")
