@@ -7,6 +7,8 @@
 //   table[b, held_b + j] = free[off_b + j], j < need_b
 //   slot[t] = table[b, p / PAGE] * PAGE + p % PAGE, with p = len_b - n_b + (t - start_b) for token t of request b
 //
+// Bound by latency: lengths -> prefix sums -> bisection -> table -> slot, one after the other, behind a launch (2.9 us from a graph for 2
+// requests, 4.8 for 300 with 77 K new tokens, 7.0 for 64 prompts of 262 K tokens; their bytes would take 0.3 at the most).
 // One launch, nothing kept between blocks: every block works the two prefix sums (pages, tokens) out for itself in shared memory
 // (a few KB of lengths out of L2), then takes its share of the tokens and of the pages handed out.  A token finds its request by
 // bisection of the starts; a page that this step hands out is read from the free list, never from the table, so that no block
@@ -18,7 +20,7 @@
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kTokensPerBlock = kThreads;       // tokens a block is launched for
+constexpr int kTokensPerBlock = kThreads;       // tokens a block is launched for (four times as many, with 64-bit divisions: 8.3 us for 300 requests, 4.8 so)
 constexpr int kMaxRequests = 16384;             // two prefix sums of 4 bytes in shared memory
 
 struct PlanArgs {

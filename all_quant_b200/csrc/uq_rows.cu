@@ -11,8 +11,10 @@
 //   split       x = hi * 2^E + lo * 2^E', hi = e4m3(x * 2^-E), lo the remainder's e4m3 with the remainder's own scale: 4 + 4
 //               significant bits hold a bf16 value exactly, save for what lies under 2^-21 of its group's largest.
 //
-// All three are bound by memory: a lane owns pieces of 8 channels (one 16-byte load of a 16-bit type), a group of 32 is four
-// lanes, whose maximum takes two shuffles; a piece leaves as one 8-byte store.
+// A lane owns pieces of 8 channels (one 16-byte load of a 16-bit type), a group of 32 is four lanes, whose maximum takes two shuffles;
+// a piece leaves as one 8-byte store.  Memory should bound all three, and does where a value brings 7 bytes (norm of 16384 x 8192 bf16 with a
+// residual: 138 us from a graph, 6.8 TB/s); with 3 and 5 bytes the issue slots run out first (norm of 8191 x 4096 fp16 23 us, 4.4 TB/s, 16
+// instructions per value; gate of 5001 x 11040 bf16 54 us, 5.1 TB/s, 24), hence the paired arithmetic.
 #include <atomic>
 #include <climits>
 
@@ -185,6 +187,7 @@ UQ_DEV void silu_mul2(float& y0, float& y1, float u0, float u1) {
   mul2(y0, y1, y0, y1, u0, u1);
 }
 
+// Five blocks per SM (us at 5001 x 11040: four 55.8, five 53.4, six 60.4; one piece in flight 55.4 to 61, four 53.4 to 61).
 // The rows' pieces are one sequence, cut into runs of a block's threads: a group's four lanes never leave their row (F is a
 // multiple of 32, runs start at multiples of 4), and no lane is idle for a row's odd end.  A thread's place moves on by
 // (step_row, step_piece), so that nothing is divided on the way.

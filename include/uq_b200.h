@@ -1,5 +1,5 @@
 /* C ABI of libuq_b200.so: paged UltraQuant FP4 verify/decode attention and KV append for NVIDIA B200
- * (sm_100a).  Plain pointers and sizes only; every function returns a cudaError_t value as int
+ * (sm_100a), and the operators that a layer's step has around them.  Plain pointers and sizes only; every function returns a cudaError_t value as int
  * (0 = success, 1 = cudaErrorInvalidValue = "this shape is not served", nothing was enqueued).
  * All launches are asynchronous on `stream` (a cudaStream_t passed as void*), allocate nothing and
  * never read device memory on the host.  Pointers are caller-owned device memory.
@@ -118,6 +118,7 @@ int uqb_silu_mul_mx8_launch(const void* x, uint8_t* codes, uint8_t* scales, long
  *   x, xs       xs NULL: x is bf16 [M, K], taken as two e4m3 planes (exact but for what lies under 2^-21 of a group's largest),
  *               scratch holds uqb_fp4_linear_scratch_bytes(M, K) bytes (none up to 4 rows: may be NULL); else x e4m3 [M, K], xs its scale bytes [M, K/32].
  *   out         [M, N], out_dtype 0 = fp32, 1 = bf16, 2 = fp16.
+ * Every wait on the device is bounded; should one run out, outputs of that call are NaN and uqb_last_status says so.
  * K a multiple of 32, wc 32-byte aligned, x / ws / out / scratch 16, xs 4.  A row of x that holds NaN or infinity (bf16), or a
  * NaN code, gives NaN in its outputs; other rows are not touched by it. */
 size_t uqb_fp4_linear_scratch_bytes(long long M, int K);
@@ -216,7 +217,8 @@ size_t uqb_static_scratch_bytes(void);
 
 /* Every device-side wait in this library is bounded; a wait that runs out records what it was
  * waiting for and the kernel returns.  Reads (and clears) the current device's record:
- * out4[0] = code (0 = none, 1 = a barrier wait of the attention kernel, 3 = a rank's flag in uqb_merge_wait_launch),
+ * out4[0] = code (0 = none, 1 = a barrier wait of the attention kernel or, with barrier ids 40-59, of uqb_fp4_linear_launch's,
+ * 3 = a rank's flag in uqb_merge_wait_launch),
  * out4[1] = block, out4[2] = barrier id (code 3: the rank), out4[3] = tile (code 3: seq).  Synchronises the device.
  * When the code is not zero, the outputs of the calls since the last read are not answers (the kernel that gave up left
  * its results unwritten or partial): from the moment the code is set until this function has read and cleared it, every

@@ -166,6 +166,26 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_kernels_keep_the_order_of_dependents():
+    """What every kernel launched as a programmatic dependent keeps to (see test_kernel_order.py): it waits before it reads or writes
+    global memory, lets its successor in only behind its own wait, takes tensor memory only there, and asks for the SM count."""
+    from tests.test_kernel_order import CSRC, kernels
+    import os
+    import re
+    seen = 0
+    for name in ("uq_plan.cu", "uq_rows.cu", "uq_linear.cu"):
+        for kernel, body in kernels(name).items():
+            seen += 1
+            waits = [m.start() for m in re.finditer(r"uq_pdl_wait\(\)", body)]
+            assert waits and body.count("uq_pdl_release()") == 1 and "__ldg" not in body, kernel
+            # (the first of two waits is that of the early exit on a misplaced buffer)
+            assert len(waits) == (2 if "linear" in kernel else 1) and body.index("uq_pdl_release()") > waits[-1], kernel
+            assert not any(what in body[:waits[-1]] for what in ("tcgen05.alloc", "tma_load", "bulk_load", ".load(", "seq_lens")), kernel
+        text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, name)).read())
+        assert "__restrict__" not in text and not re.search(r"\b148\b", text), name
+    assert seen == 6
+
+
 # ---------------------------------------------------------------------------------------------------------------- plan
 gpu = pytest.mark.gpu
 
