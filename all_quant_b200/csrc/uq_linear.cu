@@ -20,10 +20,10 @@
 // dimensions of 32 and 4 rows, the outer one first in memory), and the scale bytes are copied as they lie.
 //
 // One CTA per (128 channels, NB rows, range of K); the ranges of one tile are a cluster, each of whose CTAs adds the fp32 partial tiles
-// of all up for its share of the rows, in the order of the ranks: one launch, no scratch, the same bits every time.  Up to 32 operand
-// rows the partials are pushed: stored straight from registers into the owner's shared memory, counted on its barrier, so that nobody
-// waits for the slowest CTA twice (two cluster barriers around a pull took 1.8 of the 4.1 us of a 4-step CTA).  More rows do not fit
-// beside the ring: each CTA lays its tile out over its own ring and the owners read it between two cluster barriers.
+// of all up for its share of the rows, in the order of the ranks: one launch, no scratch, the same bits every time.  The partials are
+// pushed: stored straight from registers into the owner's shared memory and counted on its barrier (read by the owners between two
+// cluster barriers, they took 1.8 of the 4.1 us of a 4-step CTA).  Few rows have a buffer beside the ring; more go over the ring once
+// every CTA of the cluster is done with its own.
 // Two CTAs fit an SM, so that their copies overlap and a grid need not be a multiple of the SMs.
 //
 // From a graph, weights larger than L2, beside the weight's bytes at the copy rate of 6.47 TB/s: 1 x 4096 x 4096 5.0 us (1.4), 8 bf16 rows
@@ -67,14 +67,14 @@ struct LinearParams {
 template <int NB, int PLANES>
 struct LinCfg {
   static constexpr int kRows = NB / PLANES;                  // rows of x per CTA
-  static constexpr bool kPush = NB / PLANES <= 16;           // partial tiles are pushed into a buffer of their own
-  static constexpr int kStages = NB == 16 || (NB == 32 && !kPush) ? 5 : (NB <= 64 ? 4 : 3);   // what half an SM's shared memory holds
+  static constexpr bool kBeside = NB / PLANES <= 16;         // the partials' buffer lies beside the ring, not over it
+  static constexpr int kStages = NB == 16 || (NB == 32 && !kBeside) ? 5 : (NB <= 64 ? 4 : 3);   // what half an SM's shared memory holds
   static constexpr int kA = 128 * 128, kB = NB * 128, kSf = 512;
   static constexpr int oB = kA, oSfa = oB + kB, oSfb = oSfa + kSf, kStage = oSfb + kSf;
   static constexpr int kRing = kStages * kStage;
   static constexpr int kPRow = 512;                          // bytes of one row of a partial tile
-  static constexpr int kP = (kPush ? kRows + kMaxSplit - 1 : kRows) * kPRow;   // (an owner's rows x the ranks: at most that many)
-  static constexpr int oP = kPush ? kRing : 0;
+  static constexpr int kP = (kRows + kMaxSplit - 1) * kPRow;   // (an owner's rows x the ranks: at most that many)
+  static constexpr int oP = kBeside ? kRing : 0;
   static constexpr int kBody = oP + kP > kRing ? oP + kP : kRing;
   static constexpr int oBarIn = kBody, oBarTmem = oBarIn + 8, oBarW = oBarTmem + 8, oBarX = oBarW + 8 * kStages, oBarS = oBarX + 8 * kStages, oBarE = oBarS + 8 * kStages, oBarDone = oBarE + 8 * kStages;
   static constexpr int oTmem = oBarDone + 8, oAbort = oTmem + 4;
@@ -97,10 +97,6 @@ UQ_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x0, int x1, in
 }
 UQ_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 UQ_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-UQ_DEV void cluster_sync() {
-  cluster_arrive();
-  cluster_wait();
-}
 // four bytes into a CTA of the cluster, counted on the barrier there
 UQ_DEV void st_async(uint32_t addr, float v, uint32_t bar) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar) : "memory");
@@ -110,12 +106,6 @@ UQ_DEV uint32_t cluster_addr(uint32_t addr, int rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-UQ_DEV float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 // Four consecutive channels n.. of a row of N: one store where the rows' boundaries allow it, else those inside the row one by one.
 UQ_DEV void store4(float* o, const float* v, int n, int N) {
   if (N % 4 == 0) {
@@ -181,12 +171,12 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
       *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem) = kNoTmem;
     }
     __syncwarp();
-    if (C::kPush && split > 1 && lane == 0) mbar_expect_tx(bar(C::oBarIn, 0), (uint32_t)(mine * split * C::kPRow));   // (no rows: complete at once)
+    if (split > 1 && lane == 0) mbar_expect_tx(bar(C::oBarIn, 0), (uint32_t)(mine * split * C::kPRow));   // (no rows: complete at once)
   } else if (warp >= kWarpW && lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(warp < kWarpX ? &map_w : &map_x) : "memory");   // (launch arguments, not global memory)
   }
   __syncthreads();
-  if (C::kPush && split > 1) cluster_arrive();   // every CTA's barriers stand before the first push
+  if (C::kBeside && split > 1) cluster_arrive();   // every CTA's barriers stand before the first push
   uq_pdl_wait();   // from here on global memory is read and written
   if (p.pdl) uq_pdl_release();
 
@@ -331,7 +321,10 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
     const bool ok = __all_sync(0xffffffffu, wait(bar(C::oBarDone, 0), 0, 46, nk) && wait(bar(C::oBarTmem, 0), 0, 47, nk));
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
     if (ok) tc_fence_after();
-    if (C::kPush && split > 1) cluster_wait();
+    if (split > 1) {
+      if (!C::kBeside) cluster_arrive();   // this CTA's ring is free
+      cluster_wait();
+    }
     int owner = 0;
     uint32_t place = sm + C::oP + rank * C::kPRow + tid * 4;   // (row / split, rank)
 #pragma unroll
@@ -352,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = 0x7fc00000u;
       }
-      if (C::kPush && split > 1) {
+      if (split > 1) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           if (c + j < rows) st_async(cluster_addr(place, owner), __uint_as_float(v[j]), cluster_addr(bar(C::oBarIn, 0), owner));
@@ -370,17 +363,16 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   }
   __syncwarp();
   bool in = true;
-  if (C::kPush && split > 1) {
-    if (warp >= kWarpMma) cluster_wait();   // (every thread that arrived waits once)
+  if (split > 1) {
+    if (warp >= kWarpMma) {   // (every thread of the cluster takes part)
+      if (!C::kBeside) cluster_arrive();
+      cluster_wait();
+    }
     in = wait(bar(C::oBarIn, 0), 0, 48, nk);
   } else {
     __syncthreads();
-    if (!C::kPush && *abort_flag) {   // (a copy that landed late may have covered what says so)
-      for (int i = tid; i < C::kP / 4; i += kThreads) reinterpret_cast<uint32_t*>(smem_lin)[i] = 0x7fc00000u;
-      __syncthreads();
-    }
-    if (split > 1) cluster_sync();
   }
+  in = in && !*abort_flag;
   // ---- second half: this CTA's share of the rows, the partial tiles in the order of the ranks.  A warp per row, four consecutive
   // channels per lane; the loads of all ranks are issued before the first addition.
   for (int i = warp; i < mine; i += kThreads / 32) {
@@ -389,15 +381,9 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
 #pragma unroll
     for (int r = 0; r < kMaxSplit; r++)
       if (r < split) {
-        if (C::kPush || split == 1) {
-          const uint8_t* at = smem_lin + C::oP + (C::kPush ? i * split + r : t) * C::kPRow + lane * 4;
+        const uint8_t* at = smem_lin + C::oP + (i * split + r) * C::kPRow + lane * 4;
 #pragma unroll
-          for (int j = 0; j < 4; j++) u[r][j] = *reinterpret_cast<const float*>(at + j * 128);
-        } else {
-          const uint32_t at = cluster_addr(sm + C::oP + t * C::kPRow + lane * 4, r);
-#pragma unroll
-          for (int j = 0; j < 4; j++) u[r][j] = ld_cluster(at + j * 128);
-        }
+        for (int j = 0; j < 4; j++) u[r][j] = *reinterpret_cast<const float*>(at + j * 128);
       }
     float v[4] = {u[0][0], u[0][1], u[0][2], u[0][3]};
 #pragma unroll
@@ -411,8 +397,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
     else if (p.out_dtype == 1) store4(static_cast<__nv_bfloat16*>(p.out) + o, v, n, p.N);
     else store4(static_cast<__half*>(p.out) + o, v, n, p.N);
   }
-  if (!C::kPush && split > 1) cluster_sync();   // nobody leaves while its partial tile is being read
-  else __syncthreads();
+  __syncthreads();
   if (warp == kWarpMma) {
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
