@@ -30,7 +30,7 @@ def _host_command():
     inc = [os.path.join(t, "include"), os.path.join(t, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", os.path.join(CSRC, "uq_host.cpp"), "-o", HOST, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
             + [x for d in inc for x in ("-isystem", d)]
-            + [f"-L{os.path.join(t, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{os.path.join(t, 'lib')}"])
+            + [f"-L{os.path.join(t, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", f"-Wl,-rpath,{os.path.join(t, 'lib')}"])
 
 
 def build(force=False, verbose=False):

@@ -6,6 +6,7 @@
 // come from the library that uq_cuda.lib() has loaded (`bind`), so that both always are of the same build.
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -68,15 +69,18 @@ PyObject* wrap(const optional<Tensor>& t) {
 }
 void count(Py_ssize_t n, Py_ssize_t want) { REFUSE(n != want, "uq_host: ", want, " arguments"); }
 
+// A new tensor on x's device (torch's own allocator, without the way through its dispatcher).
+Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const Place& place) { return at::detail::empty_cuda(shape, type, place.device, std::nullopt); }
+
 // Outputs of 8-bit rows of n channels: allocated, or checked.
-void mx8_out(const Tensor& x, int64_t n, optional<Tensor>& codes, optional<Tensor>& scales) {
+void mx8_out(const Tensor& x, int64_t n, const Place& place, optional<Tensor>& codes, optional<Tensor>& scales) {
   c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = n;
-  if (!codes) codes = at::empty(shape, x.options().dtype(at::kFloat8_e4m3fn));
+  if (!codes) codes = fresh(shape, at::kFloat8_e4m3fn, place);
   else REFUSE(codes->scalar_type() != at::kFloat8_e4m3fn || codes->sizes() != at::IntArrayRef(shape) || !codes->is_contiguous() || (reinterpret_cast<uintptr_t>(codes->data_ptr()) & 7),
               "codes must be contiguous float8_e4m3fn of the rows' shape (8-byte aligned)");
   shape.back() = n / 32;
-  if (!scales) scales = at::empty(shape, x.options().dtype(at::kByte));
+  if (!scales) scales = fresh(shape, at::kByte, place);
   else REFUSE(scales->scalar_type() != at::kByte || scales->sizes() != at::IntArrayRef(shape) || !scales->is_contiguous(), "scales must be contiguous uint8 [..., channels / 32]");
 }
 
@@ -111,11 +115,11 @@ PyObject* plan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   REFUSE(B > 16384 || page < 1 || page > INT32_MAX || T < 0 || pages > INT32_MAX, "plan_step: at most 16384 requests, page_size >= 1, num_tokens >= 0");
   if (lens.scalar_type() != at::kInt || !lens.is_contiguous()) lens = lens.to(at::kInt).contiguous();
   if (starts && (starts->scalar_type() != at::kInt || !starts->is_contiguous())) starts = starts->to(at::kInt).contiguous();
-  if (!slots) slots = at::empty({T}, lens.options().dtype(at::kLong));
+  if (!slots) slots = fresh({T}, at::kLong, place);
   else REFUSE(slots->scalar_type() != at::kLong || slots->dim() != 1 || slots->size(0) != T || !slots->is_contiguous(), "slots must be contiguous int64 [num_tokens]");
   if (free) {
     REFUSE(free->scalar_type() != at::kInt || free->dim() != 1 || !free->is_contiguous(), "free_pages must be contiguous int32 [F]");
-    taken = at::empty({1}, lens.options());
+    taken = fresh({1}, at::kInt, place);
   }
   const c10::cuda::CUDAGuard on(place.device);
   done(plan_fn(static_cast<int32_t*>(lens.data_ptr()), static_cast<int32_t*>(ptr(starts)), (int)K, static_cast<int32_t*>(table.data_ptr()), std::max<ll>(table.stride(0), pages),
@@ -151,9 +155,9 @@ PyObject* rms_norm_mx8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (w) w = rows(*w);
   if (r) {
     r = rows(*r);
-    if (!sum) sum = at::empty(x.sizes(), x.options());
+    if (!sum) sum = fresh(x.sizes(), dt, place);
   }
-  mx8_out(x, H, codes, scales);
+  mx8_out(x, H, place, codes, scales);
   const c10::cuda::CUDAGuard on(place.device);
   done(norm_fn(x.data_ptr(), ptr(r), ptr(w), ptr(sum), static_cast<uint8_t*>(codes->data_ptr()), static_cast<uint8_t*>(scales->data_ptr()), x.numel() / H, (int)H, dtype_code(dt),
                (float)eps, stream_of(place)),
@@ -176,7 +180,7 @@ PyObject* silu_mul_mx8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t F2 = x.dim() ? x.size(-1) : 0;
   REFUSE(F2 < 64 || F2 % 64 || F2 > (1 << 21), "silu_mul_mx8: twice a multiple of 32 channels, up to 2^21 of them");
   x = rows(x);
-  mx8_out(x, F2 / 2, codes, scales);
+  mx8_out(x, F2 / 2, place, codes, scales);
   const c10::cuda::CUDAGuard on(place.device);
   done(silu_fn(x.data_ptr(), static_cast<uint8_t*>(codes->data_ptr()), static_cast<uint8_t*>(scales->data_ptr()), x.numel() / F2, (int)(F2 / 2), dtype_code(x.scalar_type()),
                stream_of(place)),
@@ -227,11 +231,11 @@ PyObject* fp4_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const ll M = x.numel() / K;
   if (!scales) {
     const int64_t need = (int64_t)scratch_fn(M, (int)K);
-    if (!work && need) work = at::empty({need}, x.options().dtype(at::kByte));
+    if (!work && need) work = fresh({need}, at::kByte, place);
     REFUSE(work && (work->scalar_type() != at::kByte || work->numel() < need || !work->is_contiguous()), "scratch too small");
   }
   shape.back() = n;
-  if (!out) out = at::empty(shape, x.options().dtype(od));
+  if (!out) out = fresh(shape, od, place);
   else REFUSE(out->scalar_type() != od || out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous(), "out must be contiguous bf16, fp16 or fp32 [..., n]");
   const c10::cuda::CUDAGuard on(place.device);
   done(linear_fn(x.data_ptr(), static_cast<uint8_t*>(ptr(scales)), static_cast<uint8_t*>(wc.data_ptr()), static_cast<uint8_t*>(ws.data_ptr()), out->data_ptr(),
