@@ -221,11 +221,18 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         *abort_flag = 1;
         uq_report(p.status, 1u, 49u, 0u);
       }
+      // The next step's barriers are looked at before this step's instructions are issued: their round trips would be most of a step.
+      int s = 0;
+      uint32_t parity = 0;
+      uint32_t have_x = mbar_test(bar(C::oBarX, 0), 0), have_s = mbar_test(bar(C::oBarS, 0), 0), have_w = mbar_test(bar(C::oBarW, 0), 0);
       for (int i = 0; i < nk && ok; i++) {
-        const int s = i % C::kStages;
-        const uint32_t parity = (i / C::kStages) & 1;
-        ok = wait(bar(C::oBarX, s), parity, 42, i) && wait(bar(C::oBarS, s), parity, 43, i) && wait(bar(C::oBarW, s), parity, 44, i);
+        ok = (have_x || wait(bar(C::oBarX, s), parity, 42, i)) && (have_s || wait(bar(C::oBarS, s), parity, 43, i)) && (have_w || wait(bar(C::oBarW, s), parity, 44, i));
         if (!ok) break;
+        const int s1 = s + 1 == C::kStages ? 0 : s + 1;
+        const uint32_t parity1 = parity ^ (s1 == 0 ? 1u : 0u);
+        have_x = mbar_test(bar(C::oBarX, s1), parity1);
+        have_s = mbar_test(bar(C::oBarS, s1), parity1);
+        have_w = mbar_test(bar(C::oBarW, s1), parity1);
         tc_fence_after();
         const uint32_t st = stage_at(s), sf = tmem + C::cSf + 8 * s;
         tmem_copy_sf(sf, sf_desc(st + C::oSfa));
@@ -234,7 +241,9 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
 #pragma unroll
         for (int kb = 0; kb < 4; kb++)
           mma_bs(tmem, a + (uint64_t)(kb * 2), b + (uint64_t)(kb * 2), instr_desc_bs(128, NB, 5, 0, kb, kb), sf, sf + 4, (i || kb) ? 1u : 0u);
-        tc_commit(bar(C::oBarE, s));
+        if (i + C::kStages < nk) tc_commit(bar(C::oBarE, s));   // (nobody waits for the last ones)
+        s = s1;
+        parity = parity1;
       }
       if (ok) tc_commit(bar(C::oBarDone, 0));
     }
@@ -527,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const _
 #pragma unroll
         for (int kb = 0; kb < 4; kb++)
           mma_bs(tmem, a + (uint64_t)(kb * 2), b + (uint64_t)(kb * 2), instr_desc_bs(128, 256, 0, 5, kb, kb), sf, sf + 4, (i || kb) ? 1u : 0u);
-        tc_commit(bar(C::oBarE, s));
+        if (i + C::kStages < nk) tc_commit(bar(C::oBarE, s));   // (nobody waits for the last ones)
       }
       if (ok) tc_commit(bar(C::oBarDone, 0));
     }
