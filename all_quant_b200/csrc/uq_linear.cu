@@ -76,8 +76,8 @@ struct LinCfg {
   static constexpr int kP = (kRows + kMaxSplit - 1) * kPRow;   // (an owner's rows x the ranks: at most that many)
   static constexpr int oP = kBeside ? kRing : 0;
   static constexpr int kBody = oP + kP > kRing ? oP + kP : kRing;
-  static constexpr int oBarIn = kBody, oBarTmem = oBarIn + 8, oBarW = oBarTmem + 8, oBarX = oBarW + 8 * kStages, oBarS = oBarX + 8 * kStages, oBarE = oBarS + 8 * kStages, oBarDone = oBarE + 8 * kStages;
-  static constexpr int oTmem = oBarDone + 8, oAbort = oTmem + 4;
+  static constexpr int oBarIn = kBody, oBarTmem = oBarIn + 8, oBarDone = oBarTmem + 8, oBarF = oBarDone + 8, oBarE = oBarF + 8 * kStages;
+  static constexpr int oTmem = oBarE + 8 * kStages, oAbort = oTmem + 4;
   static constexpr int kSmem = oAbort + 4;
   static constexpr int cSf = NB;                             // first column of the scales: 8 per stage (4 of the weight, 4 of x)
   static constexpr int kColsUsed = cSf + 8 * kStages;
@@ -155,6 +155,10 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
     return r;
   };
   const size_t block0 = (size_t)tile_n * p.ksteps + k0;   // first 128 x 128 block of this CTA's range
+  // A step's stage has one barrier for all that comes into it (weight, x with the weight's scales, x's scales): every barrier looked at
+  // costs the issuing thread 30 of the 460 cycles that a step took it with three.
+  auto full_bar = [&](int i) { return bar(C::oBarF, i % C::kStages); };
+  auto wait_free = [&](int i, int id) -> bool { return i < C::kStages || wait(bar(C::oBarE, i % C::kStages), ((i / C::kStages) & 1) ^ 1, id, i); };
   constexpr int kScaleWarps = (NB + 31) / 32;
 
   const long long m0 = (long long)tile_m * C::kRows;
@@ -162,9 +166,9 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   const int mine = (rows - rank + split - 1) / split;         // rows rank, rank + split, .. are this CTA's to add up
 
   if (warp == 0) {   // a barrier per lane
-    constexpr int kBars = 3 + 4 * C::kStages;
-    static_assert(kBars <= 32 && C::oBarX == C::oBarW + 8 * C::kStages && C::oBarDone == C::oBarW + 32 * C::kStages, "barriers lie side by side");
-    if (lane < kBars) mbar_init(sm + C::oBarIn + 8 * lane, lane >= 2 + 2 * C::kStages && lane < 2 + 3 * C::kStages ? kScaleWarps : 1);
+    constexpr int kBars = 3 + 2 * C::kStages;
+    static_assert(kBars <= 32 && C::oBarE == C::oBarIn + 8 * (3 + C::kStages), "barriers lie side by side");
+    if (lane < kBars) mbar_init(sm + C::oBarIn + 8 * lane, lane >= 3 && lane < 3 + C::kStages ? 2 + kScaleWarps : 1);
     fence_barrier_init();
     if (lane == 0) {
       *abort_flag = 0;
@@ -187,13 +191,12 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
       const uint64_t pol = l2_policy();
       uint64_t keep;
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));   // (x is read by every tile; 4096 x 4096: 5.2 us, 6.0 without)
-      const int full = weights ? C::oBarW : C::oBarX;
       int i = weights ? warp - kWarpW : warp - kWarpX;
       bool ok = true;
       for (; i < nk; i += 2) {
         const int s = i % C::kStages;
-        if (i >= C::kStages && !(ok = wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 40, i))) break;
-        const uint32_t st = stage_at(s), b = bar(full, s);
+        if (!(ok = wait_free(i, 40))) break;
+        const uint32_t st = stage_at(s), b = full_bar(i);
         if (weights) {
           mbar_expect_tx(b, 8192);   // the packed bytes are counted
           tma_load_4d(st, &map_w, 0, 0, 0, (int)(block0 + i), b, pol);
@@ -204,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         }
       }
       if (!ok)   // gave up: what this thread still has in flight lands before the CTA may end
-        for (int j = i - 2; j >= 0 && j >= i - C::kStages; j -= 2) bounded_wait(bar(full, j % C::kStages), (j / C::kStages) & 1, abort_flag, p.status, 41, j);
+        for (int j = i - 2; j >= 0 && j >= i - C::kStages; j -= 2) bounded_wait(full_bar(j), (j / C::kStages) & 1, abort_flag, p.status, 41, j);
     }
   } else if (warp == kWarpMma) {
     // (tensor memory is taken after the wait: see the verify kernel)
@@ -221,18 +224,14 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         *abort_flag = 1;
         uq_report(p.status, 1u, 49u, 0u);
       }
-      // The next step's barriers are looked at before this step's instructions are issued: their round trips would be most of a step.
+      // The next step's barrier is looked at before this step's instructions are issued.
       int s = 0;
-      uint32_t parity = 0;
-      uint32_t have_x = mbar_test(bar(C::oBarX, 0), 0), have_s = mbar_test(bar(C::oBarS, 0), 0), have_w = mbar_test(bar(C::oBarW, 0), 0);
+      uint32_t parity = 0, here = mbar_test(bar(C::oBarF, 0), 0);
       for (int i = 0; i < nk && ok; i++) {
-        ok = (have_x || wait(bar(C::oBarX, s), parity, 42, i)) && (have_s || wait(bar(C::oBarS, s), parity, 43, i)) && (have_w || wait(bar(C::oBarW, s), parity, 44, i));
-        if (!ok) break;
+        if (!here && !(ok = wait(bar(C::oBarF, s), parity, 42, i))) break;
         const int s1 = s + 1 == C::kStages ? 0 : s + 1;
         const uint32_t parity1 = parity ^ (s1 == 0 ? 1u : 0u);
-        have_x = mbar_test(bar(C::oBarX, s1), parity1);
-        have_s = mbar_test(bar(C::oBarS, s1), parity1);
-        have_w = mbar_test(bar(C::oBarW, s1), parity1);
+        here = mbar_test(bar(C::oBarF, s1), parity1);
         tc_fence_after();
         const uint32_t st = stage_at(s), sf = tmem + C::cSf + 8 * s;
         tmem_copy_sf(sf, sf_desc(st + C::oSfa));
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
           mx8::split_piece(v, hi[j], lo[j], hi_byte[j], lo_byte[j]);
         }
         load(i + 4);
-        if (i >= C::kStages && !__all_sync(0xffffffffu, wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 45, i))) break;
+        if (!__all_sync(0xffffffffu, wait_free(i, 45))) break;
         uint8_t *tile = smem_lin + s * C::kStage + C::oB, *sf = smem_lin + s * C::kStage + C::oSfb + (piece >> 2);
 #pragma unroll
         for (int j = 0; j < kPer; j++) {
@@ -292,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::oBarS, s));
+        if (lane == 0) mbar_arrive(full_bar(i));
       }
     } else {
       // ---- x's scales: thread r of a group of warps has row r's four bytes of the group's steps, two loads ahead
@@ -316,11 +315,11 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
       uint32_t w0 = load(i), w1 = load(i + kGroups);
       for (; i < nk; i += kGroups) {
         const int s = i % C::kStages;
-        if (i >= C::kStages && !__all_sync(0xffffffffu, wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 45, i))) break;
+        if (!__all_sync(0xffffffffu, wait_free(i, 45))) break;
         if (r < NB) *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfb + lane * 16 + (r >> 5) * 4) = w0;
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::oBarS, s));
+        if (lane == 0) mbar_arrive(full_bar(i));
         w0 = w1;
         w1 = load(i + 2 * kGroups);
       }
