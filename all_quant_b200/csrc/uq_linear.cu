@@ -730,7 +730,7 @@ cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8
   if (M == 0) return cudaSuccess;
   const bool direct = !xs && M <= tc::kDirectRows;
   if (!x || !wc || !ws || !out || (!xs && !direct && !scratch)) return cudaErrorInvalidValue;
-  if (!aligned_to(x, 16) || !aligned_to(wc, 32) || !aligned_to(ws, 16) || !aligned_to(out, 16) || (xs ? !aligned_to(xs, 4) : !direct && !aligned_to(scratch, 16))) return cudaErrorInvalidValue;
+  if (!aligned_to(x, 16) || !aligned_to(wc, 32) || !aligned_to(ws, 16) || !aligned_to(out, (N % 4 == 0 ? 4 : 1) * (out_dtype == 0 ? 4 : 2)) || (xs ? !aligned_to(xs, 4) : !direct && !aligned_to(scratch, 16))) return cudaErrorInvalidValue;
   const long long tiles = (N + 127) / 128, ksteps = (K + 127) / 128;
   const int planes = xs ? 1 : 2;
   const int nb = planes == 2 ? plane_tile(M) : operand_rows(M);

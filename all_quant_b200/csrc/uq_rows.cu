@@ -187,39 +187,44 @@ UQ_DEV void silu_mul2(float& y0, float& y1, float u0, float u1) {
   mul2(y0, y1, y0, y1, u0, u1);
 }
 
-// Five blocks per SM (us at 5001 x 11040: four 55.8, five 53.4, six 60.4; one piece in flight 55.4 to 61, four 53.4 to 61).
+// Five blocks per SM for 16-bit types (us at 5001 x 11040 bf16: four 55.8, five 53.4, six 60.4; one piece in flight 55.4 to 61, four 53.4 to 61).
 // The rows' pieces are one sequence, cut into runs of a block's threads: a group's four lanes never leave their row (F is a
-// multiple of 32, runs start at multiples of 4), and no lane is idle for a row's odd end.  A thread's place moves on by
-// (step_row, step_piece), so that nothing is divided on the way.
+// multiple of 32, runs start at multiples of 4), and no lane is idle for a row's odd end.  A thread's place moves on by a
+// constant number of rows and pieces, so that nothing is divided on the way.
 template <typename T>
-__global__ void __launch_bounds__(kGateThreads, 5) uq_silu_mul_kernel(GateArgs a, int pdl) {
+__global__ void __launch_bounds__(kGateThreads, sizeof(T) == 4 ? 4 : 5) uq_silu_mul_kernel(GateArgs a, int pdl) {
   uq_pdl_wait();
   if (pdl) uq_pdl_release();
   const int pieces = a.F / kPiece;
-  const long long at0 = (long long)blockIdx.x * kGateThreads + threadIdx.x;
-  long long row = at0 / pieces;
-  int p = (int)(at0 - row * pieces);
-  const long long step = (long long)gridDim.x * kGateThreads;
-  const long long step_row = step / pieces;
-  const int step_piece = (int)(step - step_row * pieces);
-  while (__any_sync(0xffffffffu, row < a.rows)) {   // (a warp's lanes leave together: the shuffles need all of them)
+  const long long all = a.rows * pieces, step = (long long)gridDim.x * kGateThreads;
+  // (the grid is no larger than what the device holds: a block's first piece and the step are small numbers)
+  const unsigned first_piece = blockIdx.x * kGateThreads + threadIdx.x, first_row = first_piece / (unsigned)pieces, step_row = (unsigned)step / (unsigned)pieces;
+  long long at = first_piece;
+  int p = (int)(first_piece - first_row * pieces);
+  const T* x = static_cast<const T*>(a.x) + (long long)first_row * 2 * a.F + p * kPiece;
+  const int step_piece = (int)((unsigned)step - step_row * pieces);
+  const long long step_x = (long long)step_row * 2 * a.F + step_piece * kPiece;
+  while (__any_sync(0xffffffffu, at < all)) {   // (a warp's lanes leave together: the shuffles need all of them)
     Raw<T> gr[kGatePieces], ur[kGatePieces];
-    long long at[kGatePieces];
+    const long long first = at;
 #pragma unroll
     for (int i = 0; i < kGatePieces; i++) {
-      at[i] = row < a.rows ? row * pieces + p : -1;
-      if (row < a.rows) {
-        const T* x = static_cast<const T*>(a.x) + row * 2 * a.F + (long long)p * kPiece;
+      if (at < all) {
         gr[i].load(x);
         ur[i].load(x + a.F);
       }
-      row += step_row;
+      at += step;
+      x += step_x;
       p += step_piece;
-      if (p >= pieces) { p -= pieces; row++; }
+      if (p >= pieces) {   // the next row: its gates begin F values behind this one's factors
+        p -= pieces;
+        x += a.F;
+      }
     }
 #pragma unroll
     for (int i = 0; i < kGatePieces; i++) {
-      const bool in = at[i] >= 0;
+      const long long here = first + i * step;
+      const bool in = here < all;
       float y[kPiece];
       if (in) {
         float u[kPiece];
@@ -231,8 +236,8 @@ __global__ void __launch_bounds__(kGateThreads, 5) uq_silu_mul_kernel(GateArgs a
       const float amax = group_amax(in ? piece_amax(y) : 0.f);
       if (in) {
         const uint32_t byte = scale_byte(amax);
-        *reinterpret_cast<uint2*>(a.codes + at[i] * kPiece) = codes_of(y, inverse_scale(byte), amax);
-        if ((threadIdx.x & 3) == 0) a.scales[at[i] >> 2] = (uint8_t)byte;
+        *reinterpret_cast<uint2*>(a.codes + here * kPiece) = codes_of(y, inverse_scale(byte), amax);
+        if ((threadIdx.x & 3) == 0) a.scales[here >> 2] = (uint8_t)byte;
       }
     }
   }

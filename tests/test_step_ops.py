@@ -138,7 +138,7 @@ def test_silu_refuses(over):
 
 
 @pytest.mark.parametrize("over", [dict(M=-1), dict(M=(1 << 24) + 1), dict(N=0), dict(K=0), dict(K=48), dict(dtype=3), dict(x=None), dict(wc=None), dict(ws=None), dict(out=None),
-                                  dict(x=_p(0, 8)), dict(wc=_p(2, 16)), dict(ws=_p(3, 8)), dict(out=_p(4, 8)), dict(xs=_p(1, 2)), dict(xs=None, scratch=None),
+                                  dict(x=_p(0, 8)), dict(wc=_p(2, 16)), dict(ws=_p(3, 8)), dict(out=_p(4, 4)), dict(xs=_p(1, 2)), dict(xs=None, scratch=None),
                                   dict(xs=None, scratch=_p(5, 8))])
 def test_linear_refuses(over):
     a = dict(x=_p(0), xs=_p(1), wc=_p(2), ws=_p(3), out=_p(4), scratch=_p(5), M=9, N=128, K=64, dtype=1)
@@ -484,6 +484,12 @@ def test_linear_rows_do_not_touch_each_other_and_nothing_beyond_is_written(M):
     assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad]) and (buf[:2] == 5).all() and (buf[M + 2:] == 5).all()
     codes, scales, _ = uq_cuda.rms_norm_mx8(x)
     assert uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales)[3].isnan().all()
+    # outputs that begin off a 16-byte boundary: rows of an odd width, and of a width that is a multiple of four
+    for n, first in ((199, 1), (196, 3)):
+        odd = torch.full((M + 4, n), 5.0, dtype=torch.bfloat16, device="cuda")
+        wn, sn = _weight(n, K, 9)
+        uq_cuda.fp4_linear(x, wn, sn, n, out=odd[first:M + first])
+        assert torch.equal(odd[first:M + first][~bad], uq_cuda.fp4_linear(x, wn, sn, n)[~bad]) and (odd[:first] == 5).all() and (odd[M + first:] == 5).all()
     # zero rows and zero values
     assert uq_cuda.fp4_linear(x[:0], wc, ws, N).shape == (0, N)
     assert (uq_cuda.fp4_linear(torch.zeros(2, 3, K, dtype=torch.bfloat16, device="cuda"), wc, ws, N) == 0).all()
