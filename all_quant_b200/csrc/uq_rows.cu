@@ -65,8 +65,7 @@ __global__ void __launch_bounds__(kOneWarp ? 128 : 1024) uq_rms_norm_kernel(Norm
   __shared__ __align__(16) float sums[32];
   const int lanes = kOneWarp ? 32 : blockDim.x;
   const int pieces = a.H / kPiece;
-  if (!kOneWarp && threadIdx.x < 32) sums[threadIdx.x] = 0.f;
-  if (!kOneWarp) __syncthreads();
+  if (!kOneWarp && threadIdx.x < 32 && threadIdx.x >= blockDim.x >> 5) sums[threadIdx.x] = 0.f;   // (read behind the barrier in row_sum)
   uq_pdl_wait();
   if (pdl) uq_pdl_release();
   const int t = kOneWarp ? (threadIdx.x & 31) : threadIdx.x;
