@@ -8,7 +8,7 @@
 //   slot[t] = table[b, p / PAGE] * PAGE + p % PAGE, with p = len_b - n_b + (t - start_b) for token t of request b
 //
 // Bound by latency: lengths -> prefix sums -> bisection -> table -> slot, one after the other, behind a launch (2.9 us from a graph for 2
-// requests, 4.8 for 300 with 77 K new tokens, 7.0 for 64 prompts of 262 K tokens; their bytes would take 0.3 at the most).
+// requests, 4.7 for 300 with 77 K new tokens, 6.6 for 64 prompts of 295 K tokens; their bytes would take 0.3 at the most).
 // One launch, nothing kept between blocks: every block works the two prefix sums (pages, tokens) out for itself in shared memory
 // (a few KB of lengths out of L2), then takes its share of the tokens and of the pages handed out.  A token finds its request by
 // bisection of the starts; a page that this step hands out is read from the free list, never from the table, so that no block
@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kTokensPerBlock = kThreads;       // tokens a block is launched for (four times as many, with 64-bit divisions: 8.3 us for 300 requests, 4.8 so)
-constexpr int kMaxRequests = 16384;             // two prefix sums of 4 bytes in shared memory
+constexpr int kMaxRequests = 16384;             // two prefix sums and a position of 4 bytes each in shared memory
 
 struct PlanArgs {
   const int32_t* seq_lens;    // [B]
@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(kThreads) uq_plan_kernel(PlanArgs a, int pdl) 
   extern __shared__ int sm[];
   int* off = sm;                  // [B + 1] pages handed out before request b
   int* first = sm + a.B + 1;      // [B + 1] first new token of request b
+  int* behind = first + a.B + 1;  // [B] its position: what was stored before (below zero: more new tokens than stored ones)
   __shared__ long long sums[kThreads / 32];
   const int tid = threadIdx.x;
   uq_pdl_wait();
@@ -101,6 +102,7 @@ __global__ void __launch_bounds__(kThreads) uq_plan_kernel(PlanArgs a, int pdl) 
       request(a, b, len, n);
       off[b] = saturate(pages);
       first[b] = a.starts ? a.starts[b] : saturate(tokens);
+      behind[b] = (int)max((long long)len - n, (long long)INT_MIN);
       pages += max(pages_of(len, a.PAGE, a.max_pages) - pages_of((long long)len - n, a.PAGE, a.max_pages), 0);
       tokens += n;
     }
@@ -115,13 +117,12 @@ __global__ void __launch_bounds__(kThreads) uq_plan_kernel(PlanArgs a, int pdl) 
     int64_t slot = -1;
     if (t >= first[0] && t < first[a.B]) {
       const int b = last_not_above(first, a.B - 1, (int)t);
-      int len, n;
-      request(a, b, len, n);
-      const long long pos = (long long)len - n + (t - first[b]);
-      if (pos >= 0 && pos < len) {
+      const long long i = t - first[b], pos = (long long)behind[b] + i;
+      // (starts that fall are no starts: such a request has no tokens, whatever lies between it and the next)
+      if (pos >= 0 && i < (a.K > 0 ? (long long)a.K : (long long)first[b + 1] - first[b])) {
         const int pi = (int)((unsigned)pos / (unsigned)a.PAGE);
         if (pi < a.max_pages) {
-          const int held = pages_of((long long)len - n, a.PAGE, a.max_pages);
+          const int held = pages_of(behind[b], a.PAGE, a.max_pages);
           int page = -1;
           if (pi < held || !a.taken) page = a.table[b * a.stride + pi];
           else {
@@ -138,9 +139,7 @@ __global__ void __launch_bounds__(kThreads) uq_plan_kernel(PlanArgs a, int pdl) 
     const int total = off[a.B];
     for (long long i = (long long)blockIdx.x * kThreads + tid; i < total; i += step) {
       const int b = last_not_above(off, a.B - 1, (int)i);
-      int len, n;
-      request(a, b, len, n);
-      a.table[b * a.stride + pages_of((long long)len - n, a.PAGE, a.max_pages) + ((int)i - off[b])] = i < a.n_free ? a.free_pages[i] : -1;
+      a.table[b * a.stride + pages_of(behind[b], a.PAGE, a.max_pages) + ((int)i - off[b])] = i < a.n_free ? a.free_pages[i] : -1;
     }
     if (blockIdx.x == 0 && tid == 0) *a.taken = total;
   }
@@ -152,14 +151,14 @@ cudaError_t uq_plan_dispatch(const int32_t* seq_lens, const int32_t* starts, int
                              int64_t* slots, int32_t* taken, int B, long long T, int PAGE, int max_pages, int sms, cudaStream_t s) {
   if (B < 0 || B > kMaxRequests || K < 0 || (K > 0 && starts) || T < 0 || T > INT_MAX || PAGE < 1 || max_pages < 0 || n_free < 0 || stride < max_pages) return cudaErrorInvalidValue;
   if ((long long)B * max_pages > INT_MAX || (B > 0 && (!seq_lens || (max_pages > 0 && !table))) || (T > 0 && !slots) || (n_free > 0 && (!free_pages || !taken))) return cudaErrorInvalidValue;
-  const size_t smem = 2 * (size_t)(B + 1) * sizeof(int);
+  const size_t smem = 3 * (size_t)(B + 1) * sizeof(int);
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(uq_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * (kMaxRequests + 1) * sizeof(int)));
+    const cudaError_t e = cudaFuncSetAttribute(uq_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(3 * (kMaxRequests + 1) * sizeof(int)));
     if (e != cudaSuccess) { cudaGetLastError(); return e; }
   }
   PlanArgs a{seq_lens, starts, table, free_pages, slots, taken, stride, T, n_free, B, K, PAGE, max_pages};
   const long long want = (T + kTokensPerBlock - 1) / kTokensPerBlock;
-  const unsigned blocks = (unsigned)(want < 1 ? 1 : (want > 2 * sms ? 2 * sms : want));
+  const unsigned blocks = (unsigned)(want < 1 ? 1 : (want > 4 * sms ? 4 * sms : want));
   const bool pdl = uq_pdl_on();
   return uq_launch(uq_plan_kernel, dim3(blocks), (unsigned)kThreads, smem, s, pdl, a, (int)pdl);
 }
