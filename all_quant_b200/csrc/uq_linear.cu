@@ -26,8 +26,8 @@
 // every CTA of the cluster is done with its own.
 // Two CTAs fit an SM, so that their copies overlap and a grid need not be a multiple of the SMs.
 //
-// From a graph, weights larger than L2, beside the weight's bytes at the copy rate of 6.47 TB/s: 1 x 4096 x 4096 5.0 us (1.4), 8 bf16 rows
-// x 10240 x 8192 13.7 (6.9), 17 8-bit rows x 8192 x 32768 26 (22), 1 x 65536 x 8192 48 (44), 64 bf16 rows x 65536 x 8192 70 (44).  Fill and drain are
+// From a graph, weights larger than L2, beside the weight's bytes at the copy rate of 6.47 TB/s: 1 x 4096 x 4096 4.8 us (1.4), 8 bf16 rows
+// x 10240 x 8192 13.4 (6.9), 17 8-bit rows x 8192 x 32768 25.6 (22), 1 x 65536 x 8192 47.6 (44), 64 bf16 rows x 65536 x 8192 68 to 71 (44).  Fill and drain are
 // about 4 us of each: launch, first copies (1 us), the cluster's sum, and CTAs that start late because the last call's still hold an SM's halves.
 #include <climits>
 
@@ -160,6 +160,8 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   // A step's stage has one barrier for all that comes into it (weight, x with the weight's scales, x's scales): every barrier looked at
   // costs the issuing thread 30 of the 460 cycles that a step took it with three.
   auto full_bar = [&](int i) { return bar(C::oBarF, i % C::kStages); };
+  // (A wait by parity tells a phase from its neighbours only: the warps of a role that take turns are no more than the stages, so that
+  // a warp's step before this one has seen the phase before the one that it now waits for.)
   auto wait_free = [&](int i, int id) -> bool { return i < C::kStages || wait(bar(C::oBarE, i % C::kStages), ((i / C::kStages) & 1) ^ 1, id, i); };
   constexpr int kScaleWarps = (NB + 31) / 32;
 
@@ -253,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
       // ---- x itself: a warp splits a step's 4 rows x 128 channels (lane: piece lane % 16 of rows lane / 16 and 2 + lane / 16) into the two planes of the
       // tile, rows r and 8 + r of 128 bytes with the 128-byte swizzle, and their scale bytes; the next step's loads are on their way.
       static_assert(!kDirect || (NB == 16 && PLANES == 2), "rows of both planes");
+      static_assert(4 <= C::kStages, "four warps take turns");
       constexpr int kPer = kDirectRows / 2;   // pieces of a lane
       const int piece = lane & 15, r0 = lane >> 4;
       mx8::Raw<__nv_bfloat16> next[kPer];
@@ -298,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
     } else {
       // ---- x's scales: thread r of a group of warps has row r's four bytes of the group's steps, two loads ahead
       constexpr int kGroups = 4 / kScaleWarps;
+      static_assert(kGroups <= C::kStages && 2 <= C::kStages, "as many warps take turns");
       const int r = (warp % kScaleWarps) * 32 + lane, groups = p.K / 32;
       const long long row = (long long)tile_m * NB + r;
       const bool have = r < NB && row < p.xrows;
