@@ -451,6 +451,32 @@ def test_linear_long_and_wide(M, N, K):
 
 
 @gpu
+def test_linear_many_rows_and_one():
+    """More rows than any tile holds, and no row axis at all."""
+    N, K = 384, 512
+    wc, ws = _weight(N, K, 5)
+    w64 = weight64(wc, ws, N, K)
+    x = _rand((1000, K), torch.bfloat16, 6)
+    check_linear(uq_cuda.fp4_linear(x, wc, ws, N), _f64(x), w64, torch.bfloat16, split=True)
+    codes, scales, s = uq_cuda.rms_norm_mx8(x, None, x)
+    check_linear(uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales), mx8_values(codes, scales), w64, torch.bfloat16)
+    one, one_s, s1 = uq_cuda.rms_norm_mx8(x[7], None, x[7])
+    assert one.shape == (K,) and one_s.shape == (K // 32,) and torch.equal(s1, s[7])
+    assert torch.equal(one.view(torch.uint8), codes[7].view(torch.uint8)) and torch.equal(one_s, scales[7])
+    y = uq_cuda.fp4_linear(one, wc, ws, N, scales=one_s, out_dtype=torch.float32)
+    assert y.shape == (N,)
+    check_linear(y[None], mx8_values(one, one_s)[None], w64, torch.float32)
+    assert uq_cuda.fp4_linear(x[7], wc, ws).shape == (N,) and uq_cuda.silu_mul_mx8(x[7])[0].shape == (K // 2,)
+    # rows that are not contiguous, codes and scales alike
+    wide = torch.zeros(20, 2 * K, dtype=torch.uint8, device="cuda")
+    wide[:, :K] = codes[:20].view(torch.uint8)
+    wide_s = torch.zeros(K // 32, 20, dtype=torch.uint8, device="cuda")
+    wide_s.copy_(scales[:20].t())
+    got = uq_cuda.fp4_linear(wide[:, :K].view(torch.float8_e4m3fn), wc, ws, N, scales=wide_s.t())
+    assert torch.equal(got, uq_cuda.fp4_linear(codes[:20].contiguous(), wc, ws, N, scales=scales[:20].contiguous()))
+
+
+@gpu
 def test_linear_every_code_and_scale():
     """All sixteen codes against all 256 e4m3 values, and scales over the whole range that products of fp32 hold."""
     wc = torch.arange(256, dtype=torch.uint8, device="cuda").repeat(1, 1, 32, 1).view(1, 1, 128, 64).contiguous()
@@ -698,3 +724,30 @@ def test_a_captured_step_follows_growing_requests():
         n, used = n + K, used + t
         torch.cuda.synchronize()
         assert slots.tolist() == want_slots.tolist() and int(taken) == t and (table.cpu().numpy() == want).all()
+
+
+@gpu
+def test_ordinary_launches_give_the_same_bits(tmp_path):
+    """UQ_B200_CFG=pdl=0 (read at a process's first launch): every launch an ordinary one."""
+    import os
+    import subprocess
+    import sys
+    from tests.conftest import ROOT
+    code = """
+import sys, torch
+from all_quant_b200 import uq_cuda as U
+g = torch.Generator(device="cuda").manual_seed(3)
+x, r = (torch.randn(40, 1056, generator=g, device="cuda").bfloat16() for _ in range(2))
+wc, ws = U.pack_fp4_weight(torch.randn(700, 1056, generator=g, device="cuda"))
+c, s, t = U.rms_norm_mx8(x, None, r)
+out = [c.view(torch.uint8), s, t, U.fp4_linear(c, wc, ws, 700, scales=s), U.fp4_linear(t, wc, ws, 700), U.fp4_linear(t[:3], wc, ws, 700), *(o.view(torch.uint8) for o in U.silu_mul_mx8(t[:, :1024]))]
+bt = torch.full((2, 8), 5, dtype=torch.int32, device="cuda")
+out += [*U.plan_step(torch.tensor([40, 17], dtype=torch.int32, device="cuda"), 9, bt, 16, 20, free_pages=torch.arange(9, dtype=torch.int32, device="cuda")), bt]
+torch.save([o.cpu() for o in out], sys.argv[1])
+"""
+    results = []
+    for cfg in ("", "pdl=0"):
+        path = str(tmp_path / ("out" + cfg))
+        subprocess.run([sys.executable, "-c", code, path], check=True, cwd=ROOT, env=dict(os.environ, UQ_B200_CFG=cfg), timeout=300)
+        results.append(torch.load(path))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
