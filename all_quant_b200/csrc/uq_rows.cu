@@ -246,8 +246,10 @@ __global__ void __launch_bounds__(kGateThreads, sizeof(T) == 4 ? 4 : 5) uq_silu_
 // Rows are laid out as uq_linear.cu reads them: tiles of tile_rows rows, a tile's leading planes, then its remainder planes; what
 // fills up the last tile is never written, its products never read.
 __global__ void __launch_bounds__(kGateThreads) uq_split_kernel(const __nv_bfloat16* x, uint8_t* codes, uint8_t* scales, long long rows, int K, int tile_rows, int pdl) {
-  uq_pdl_wait();
+  // Released before its own wait, unlike the others: what follows is always the products' kernel of the same call, which lets nobody in before
+  // this one is done, and may set its CTAs up meanwhile (8 rows x 4096 x 4096 6.62 -> 6.28 us, x 10240 x 8192 13.4 -> 13.2).
   if (pdl) uq_pdl_release();
+  uq_pdl_wait();
   const int pieces = K / kPiece;
   const int p = blockIdx.x * kGateThreads + threadIdx.x;
   const bool in = p < pieces;

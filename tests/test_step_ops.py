@@ -168,7 +168,7 @@ def test_cpu_tensors_are_refused():
 
 def test_kernels_keep_the_order_of_dependents():
     """What every kernel launched as a programmatic dependent keeps to (see test_kernel_order.py): it waits before it reads or writes
-    global memory, lets its successor in only behind its own wait, takes tensor memory only there, and asks for the SM count."""
+    global memory, lets its successor in only behind its own wait (but for one), takes tensor memory only there, and asks for the SM count."""
     from tests.test_kernel_order import CSRC, kernels
     import os
     import re
@@ -179,7 +179,9 @@ def test_kernels_keep_the_order_of_dependents():
             waits = [m.start() for m in re.finditer(r"uq_pdl_wait\(\)", body)]
             assert waits and body.count("uq_pdl_release()") == 1 and "__ldg" not in body, kernel
             # (the first of two waits is that of the early exit on a misplaced buffer)
-            assert len(waits) == (2 if "linear" in kernel else 1) and body.index("uq_pdl_release()") > waits[-1], kernel
+            assert len(waits) == (2 if "linear" in kernel else 1), kernel
+            # (the split of rows, which only the products' kernel of the same call follows, lets that set itself up early)
+            assert (body.index("uq_pdl_release()") > waits[-1]) == ("split" not in kernel), kernel
             assert not any(what in body[:waits[-1]] for what in ("tcgen05.alloc", "tma_load", "bulk_load", ".load(", "seq_lens")), kernel
         text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, name)).read())
         assert "__restrict__" not in text and not re.search(r"\b148\b", text), name
