@@ -62,6 +62,7 @@ struct LinearParams {
   int out_dtype;
   int words;            // x's scale bytes of 128 channels are aligned words
   int pdl;
+  int expire;           // for the test of the give-up path: the first step's scales of x are never announced
 };
 
 template <int NB, int PLANES>
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(full_bar(i));
+        if (lane == 0 && (i > 0 || !p.expire)) mbar_arrive(full_bar(i));
       }
     } else {
       // ---- x's scales: thread r of a group of warps has row r's four bytes of the group's steps, two loads ahead
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         if (r < NB) *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfb + lane * 16 + (r >> 5) * 4) = w0;
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(full_bar(i));
+        if (lane == 0 && (i > 0 || !p.expire)) mbar_arrive(full_bar(i));
         w0 = w1;
         w1 = load(i + 2 * kGroups);
       }
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const _
         *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfx + lane * 16 + warp * 4) = w0;
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::oBarS, s));
+        if (lane == 0 && (i > 0 || !p.expire)) mbar_arrive(bar(C::oBarS, s));
         w0 = w1;
         w1 = load(i + 2);
       }
@@ -728,7 +729,7 @@ size_t uq_fp4_linear_scratch(long long M, int K) { return M <= tc::kDirectRows |
 // xs null: x is bf16 [M, K], scratch holds uq_fp4_linear_scratch bytes; else x is e4m3 [M, K] with scale bytes xs [M, K / 32].
 // launches: kernels enqueued.
 cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, void* out, void* scratch, long long M, int N, int K, int out_dtype,
-                                   unsigned int* status, int sms, cudaStream_t s, int* launches) {
+                                   unsigned int* status, int sms, bool expire, cudaStream_t s, int* launches) {
   *launches = 0;
   if (M < 0 || M > (1 << 24) || N < 1 || N > (1 << 24) || K < 32 || K > (1 << 24) || K % 32 || out_dtype < 0 || out_dtype > 2) return cudaErrorInvalidValue;
   if (M == 0) return cudaSuccess;
@@ -770,6 +771,7 @@ cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8
   p.out_dtype = out_dtype;
   p.words = K % 128 == 0 && aligned_to(p.xs, 4);
   p.pdl = uq_pdl_on() ? 1 : 0;
+  p.expire = expire;
   p.tiles = (int)tiles;
   // 128 operand rows: 256 channels a CTA where the tiles are more than the SMs (64 bf16 rows, us with 128 / 256 channels: 14336 x 4096
   // 16.5 / 18.2, 16384 x 8192 24.5 / 31.1, 20000 x 4096 22.9 / 18.6, 28672 x 8192 39.8 / 33.9, 65536 x 8192 83 / 72; 128 8-bit rows,

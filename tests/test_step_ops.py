@@ -753,3 +753,25 @@ torch.save([o.cpu() for o in out], sys.argv[1])
         subprocess.run([sys.executable, "-c", code, path], check=True, cwd=ROOT, env=dict(os.environ, UQ_B200_CFG=cfg), timeout=300)
         results.append(torch.load(path))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K,bf16", [(3, 256, 1024, True), (20, 256, 2048, False), (64, 300, 1024, True), (64, 19100, 256, True)])
+def test_a_wait_that_runs_out_shows_in_the_output_and_the_next_call_is_right(M, N, K, bf16, monkeypatch):
+    """The give-up path on a healthy GPU: with UQ_B200_CFG=expire=42 the first step's scales of x are never announced, so the issuing
+    thread's wait for them - bounded at one second, like every wait - runs out.  The kernel returns (all roles drain, TMEM goes back), its
+    outputs are NaN, the status record names a wait of these kernels, and the next call is right."""
+    wc, ws = _weight(N, K, 8)
+    x = _rand((M, K), torch.bfloat16, 8)
+    codes, scales, _ = uq_cuda.rms_norm_mx8(x)
+    call = (lambda: uq_cuda.fp4_linear(x, wc, ws, N)) if bf16 else (lambda: uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales))
+    want = call()
+    assert uq_cuda.last_status() == (0, 0, 0, 0) and not want.isnan().any()
+    monkeypatch.setenv("UQ_B200_CFG", "expire=42")
+    assert call().isnan().all()
+    st = uq_cuda.last_status()
+    assert st[0] == 1 and 40 <= st[2] < 60, st
+    monkeypatch.delenv("UQ_B200_CFG")
+    for _ in range(2):
+        assert torch.equal(call(), want)
+        assert uq_cuda.last_status() == (0, 0, 0, 0)
