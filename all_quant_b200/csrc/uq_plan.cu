@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kTokensPerBlock = kThreads;       // tokens a block is launched for (four times as many, with 64-bit divisions: 8.3 us for 300 requests, 4.8 so)
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRequests = 16384;             // two prefix sums and a position of 4 bytes each in shared memory
 
 struct PlanArgs {
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(kThreads) uq_plan_kernel(PlanArgs a, int pdl) 
   int* off = sm;                  // [B + 1] pages handed out before request b
   int* first = sm + a.B + 1;      // [B + 1] first new token of request b
   int* behind = first + a.B + 1;  // [B] its position: what was stored before (below zero: more new tokens than stored ones)
-  __shared__ long long sums[kThreads / 32];
+  __shared__ long long sums[kWarps];
   const int tid = threadIdx.x;
   uq_pdl_wait();
   if (pdl) uq_pdl_release();
@@ -152,7 +153,7 @@ cudaError_t uq_plan_dispatch(const int32_t* seq_lens, const int32_t* starts, int
   if (B < 0 || B > kMaxRequests || K < 0 || (K > 0 && starts) || T < 0 || T > INT_MAX || PAGE < 1 || max_pages < 0 || n_free < 0 || stride < max_pages) return cudaErrorInvalidValue;
   if ((long long)B * max_pages > INT_MAX || (B > 0 && (!seq_lens || (max_pages > 0 && !table))) || (T > 0 && !slots) || (n_free > 0 && (!free_pages || !taken))) return cudaErrorInvalidValue;
   const size_t smem = 3 * (size_t)(B + 1) * sizeof(int);
-  if (smem > 48 * 1024) {
+  if (smem + kWarps * sizeof(long long) > 48 * 1024) {   // what a launch gets unasked holds the warps' sums as well
     const cudaError_t e = cudaFuncSetAttribute(uq_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(3 * (kMaxRequests + 1) * sizeof(int)));
     if (e != cudaSuccess) { cudaGetLastError(); return e; }
   }

@@ -775,3 +775,25 @@ def test_a_wait_that_runs_out_shows_in_the_output_and_the_next_call_is_right(M, 
     for _ in range(2):
         assert torch.equal(call(), want)
         assert uq_cuda.last_status() == (0, 0, 0, 0)
+
+
+# ------------------------------------------------------------------------------------------------- edges of what is served
+@gpu
+def test_plan_around_the_default_size_of_shared_memory(tmp_path):
+    """Three words of shared memory per request and the warps' sums: from B = 4085 on a launch has to ask for more than it gets unasked.  In a
+    process of its own and in rising order, since a larger call raises the limit for those after it."""
+    import subprocess
+    import sys
+    from tests.conftest import ROOT
+    code = """
+import numpy as np, torch
+from all_quant_b200 import uq_cuda as U
+for B in (4083, 4084, 4085, 4090, 4095, 4096, 16384):
+    lens = np.random.default_rng(B).integers(1, 40, B)
+    table, free = torch.full((B, 3), 5, dtype=torch.int32, device="cuda"), torch.arange(100, 100 + 3 * B, dtype=torch.int32, device="cuda")
+    slots, taken = U.plan_step(torch.from_numpy(lens.astype(np.int32)).cuda(), 1, table, 16, B, free_pages=free)
+    new, page = (lens - 1) % 16 == 0, np.full(B, 5)
+    page[new] = 100 + np.arange(new.sum())
+    assert int(taken) == new.sum() and (slots.cpu().numpy() == page * 16 + (lens - 1) % 16).all(), B
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT, timeout=300)
