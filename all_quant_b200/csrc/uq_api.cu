@@ -46,7 +46,7 @@ cudaError_t uq_plan_dispatch(const int32_t*, const int32_t*, int, int32_t*, long
 cudaError_t uq_rms_norm_dispatch(const void*, const void*, const void*, void*, uint8_t*, uint8_t*, long long, int, int, float, int sms, cudaStream_t);
 cudaError_t uq_silu_mul_dispatch(const void*, uint8_t*, uint8_t*, long long, int, int, int sms, cudaStream_t);
 size_t uq_fp4_linear_scratch(long long, int);
-cudaError_t uq_fp4_linear_dispatch(const void*, const uint8_t*, const uint8_t*, const uint8_t*, void*, void*, long long, int, int, int, unsigned int* status, int sms, bool expire, cudaStream_t, int* launches);
+cudaError_t uq_fp4_linear_dispatch(const void*, const uint8_t*, const uint8_t*, const uint8_t*, void*, void*, long long, int, int, int, unsigned int* status, int sms, int expire, cudaStream_t, int* launches);
 
 namespace {
 
@@ -74,7 +74,7 @@ bool aligned(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>
 // UQ_B200_CFG="expire=30" makes the tcgen05 kernel's softmax role withhold one arrival (the query tile of a segment is never
 // announced), so that the issuing thread's bounded wait on barrier 30 runs out after its second and the kernel's give-up path
 // (status record, drain of the copies in flight, common exit) runs on a healthy GPU; "expire=42" does the same in the products' kernels (the
-// first step's scales of x).  Tests only.
+// first step's scales of x), "expire=43" in the last CTA of every cluster only.  Tests only.
 int forced_expire() {
   const char* e = std::getenv("UQ_B200_CFG");
   const char* at = e ? std::strstr(e, "expire=") : nullptr;
@@ -332,7 +332,8 @@ int uqb_fp4_linear_launch(const void* x, const uint8_t* xs, const uint8_t* wc, c
                           void* stream) {
   unsigned int* status = status_ptr();
   int launches = 0;
-  cudaError_t e = uq_fp4_linear_dispatch(x, xs, wc, ws, out, scratch, M, N, K, out_dtype, status, sm_count(), forced_expire() == 42, reinterpret_cast<cudaStream_t>(stream),
+  const int expire = forced_expire();
+  cudaError_t e = uq_fp4_linear_dispatch(x, xs, wc, ws, out, scratch, M, N, K, out_dtype, status, sm_count(), expire == 42 ? 1 : (expire == 43 ? 2 : 0), reinterpret_cast<cudaStream_t>(stream),
                                          &launches);
   g_launches += (unsigned)launches;
   return (int)e;

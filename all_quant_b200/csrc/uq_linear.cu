@@ -62,7 +62,7 @@ struct LinearParams {
   int out_dtype;
   int words;            // x's scale bytes of 128 channels are aligned words
   int pdl;
-  int expire;           // for the test of the give-up path: the first step's scales of x are never announced
+  int expire;           // for the test of the give-up path: the first step's scales of x are never announced (1: by any CTA, 2: by the last of each cluster)
 };
 
 template <int NB, int PLANES>
@@ -80,7 +80,7 @@ struct LinCfg {
   static constexpr int oP = kBeside ? kRing : 0;
   static constexpr int kBody = oP + kP > kRing ? oP + kP : kRing;
   static constexpr int oBarIn = kBody, oBarTmem = oBarIn + 8, oBarDone = oBarTmem + 8, oBarF = oBarDone + 8, oBarE = oBarF + 8 * kStages;
-  static constexpr int oTmem = oBarE + 8 * kStages, oAbort = oTmem + 4;
+  static constexpr int oBarLast = oBarE + 8 * kStages, oTmem = oBarLast + 8, oAbort = oTmem + 4;
   static constexpr int kSmem = oAbort + 4;
   static constexpr int cSf = NB;                             // first column of the scales: 8 per stage (4 of the weight, 4 of x)
   static constexpr int kColsUsed = cSf + 8 * kStages;
@@ -169,9 +169,10 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   const long long m0 = (long long)tile_m * C::kRows;
   const int rows = (int)min((long long)C::kRows, p.M - m0);   // of this tile
   const int mine = (rows - rank + split - 1) / split;         // rows rank, rank + split, .. are this CTA's to add up
+  const bool expire = p.expire == 1 || (p.expire == 2 && rank == split - 1);
 
   if (warp == 0) {   // a barrier per lane
-    constexpr int kBars = 3 + 2 * C::kStages;
+    constexpr int kBars = 4 + 2 * C::kStages;
     static_assert(kBars <= 32 && C::oBarE == C::oBarIn + 8 * (3 + C::kStages), "barriers lie side by side");
     if (lane < kBars) mbar_init(sm + C::oBarIn + 8 * lane, lane >= 3 && lane < 3 + C::kStages ? 2 + kScaleWarps : 1);
     fence_barrier_init();
@@ -189,6 +190,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   uq_pdl_wait();   // from here on global memory is read and written
   if (p.pdl) uq_pdl_release();
 
+  int issued = 0;   // by a copying thread: every other step below it
   if (warp >= kWarpW) {
     // ---- copies: two threads each for the weight's codes, and for x with the weight's scales
     if (elect_one()) {
@@ -197,10 +199,9 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
       uint64_t keep;
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));   // (x is read by every tile; 4096 x 4096: 5.2 us, 6.0 without)
       int i = weights ? warp - kWarpW : warp - kWarpX;
-      bool ok = true;
       for (; i < nk; i += 2) {
         const int s = i % C::kStages;
-        if (!(ok = wait_free(i, 40))) break;
+        if (!wait_free(i, 40)) break;
         const uint32_t st = stage_at(s), b = full_bar(i);
         if (weights) {
           mbar_expect_tx(b, 8192);   // the packed bytes are counted
@@ -211,8 +212,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
           bulk_load(st + C::oSfa, p.ws + (block0 + i) * 512, 512, b, pol);
         }
       }
-      if (!ok)   // gave up: what this thread still has in flight lands before the CTA may end
-        for (int j = i - 2; j >= 0 && j >= i - C::kStages; j -= 2) bounded_wait(full_bar(j), (j / C::kStages) & 1, abort_flag, p.status, 41, j);
+      issued = i;
     }
   } else if (warp == kWarpMma) {
     // (tensor memory is taken after the wait: see the verify kernel)
@@ -249,7 +249,12 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         s = s1;
         parity = parity1;
       }
-      if (ok) tc_commit(bar(C::oBarDone, 0));
+      if (ok) {
+        tc_commit(bar(C::oBarDone, 0));
+      } else if (tmem != kNoTmem) {   // gave up: what has been issued ends before tensor memory goes back
+        tc_commit(bar(C::oBarLast, 0));
+        ended_wait(bar(C::oBarLast, 0), 0);
+      }
     }
   } else {
     if constexpr (kDirect) {
@@ -297,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0 && (i > 0 || !p.expire)) mbar_arrive(full_bar(i));
+        if (lane == 0 && (i > 0 || !expire)) mbar_arrive(full_bar(i));
       }
     } else {
       // ---- x's scales: thread r of a group of warps has row r's four bytes of the group's steps, two loads ahead
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         if (r < NB) *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfb + lane * 16 + (r >> 5) * 4) = w0;
         fence_async_smem();
         __syncwarp();
-        if (lane == 0 && (i > 0 || !p.expire)) mbar_arrive(full_bar(i));
+        if (lane == 0 && (i > 0 || !expire)) mbar_arrive(full_bar(i));
         w0 = w1;
         w1 = load(i + 2 * kGroups);
       }
@@ -417,6 +422,12 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
     if (tmem != kNoTmem) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kCols) : "memory");
+  } else if (*abort_flag) {
+    // Somebody here gave up, and the CTA ends behind all that reaches its shared memory.  Pushes: it is sent all of them, and soon, since a CTA that gives up
+    // pushes NaN behind its last limited wait (a barrier of the whole cluster at the end of every call instead: 0.14 us).  Copies: the stages' last
+    // turns, and those before them, of which nobody may have taken notice (where such a stage has been filled again, the wait runs out).
+    if (split > 1) ended_wait(bar(C::oBarIn, 0), 0);
+    for (int j = issued - 2; j >= 0 && j >= issued - 2 * C::kStages; j -= 2) wait(full_bar(j), (j / C::kStages) & 1, 41, j);
   }
 }
 
@@ -437,7 +448,7 @@ struct WideCfg {
   static constexpr int kRing = kStages * kStage;
   static constexpr int kPRow = 257 * 4;                             // bytes of a row of the result, one per operand row (odd in words: a lane per row writes it)
   static constexpr int oBarDone = kRing, oBarTmem = oBarDone + 8, oBarW = oBarTmem + 8, oBarX = oBarW + 8 * kStages, oBarS = oBarX + 8 * kStages, oBarE = oBarS + 8 * kStages;
-  static constexpr int oTmem = oBarE + 8 * kStages, oAbort = oTmem + 4;
+  static constexpr int oBarLast = oBarE + 8 * kStages, oTmem = oBarLast + 8, oAbort = oTmem + 4;
   static constexpr int kSmem = oAbort + 4;
   static constexpr int cSf = 256, kCols = 512;                      // columns of the scales: 12 per stage (4 of x, 8 of the weight)
   static_assert(128 * kPRow <= kRing && cSf + 12 * kStages <= kCols && kSmem + 1024 <= 228 * 1024, "fits an SM");
@@ -470,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const _
   const size_t block[2] = {(size_t)(2 * pair) * nk, (size_t)min(2 * pair + 1, p.tiles - 1) * nk};
 
   if (warp == 0) {   // a barrier per lane
-    constexpr int kBars = 2 + 4 * C::kStages;
+    constexpr int kBars = 3 + 4 * C::kStages;
     static_assert(kBars <= 32 && C::oBarE == C::oBarDone + 8 * (2 + 3 * C::kStages), "barriers lie side by side");
     if (lane < kBars) mbar_init(sm + C::oBarDone + 8 * lane, lane < 2 || lane >= 2 + 3 * C::kStages ? 1 : (lane < 2 + 2 * C::kStages ? 2 : 4));
     fence_barrier_init();
@@ -494,10 +505,9 @@ __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const _
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
       const int full = role < 2 ? C::oBarW : C::oBarX;
       int i = 0;
-      bool ok = true;
       for (; i < nk; i++) {
         const int s = i % C::kStages;
-        if (i >= C::kStages && !(ok = wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 50, i))) break;
+        if (i >= C::kStages && !wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 50, i)) break;
         const uint32_t st = stage_at(s), b = bar(full, s);
         if (role < 2) {
           mbar_expect_tx(b, 8192);   // the packed bytes are counted
@@ -511,8 +521,8 @@ __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const _
           bulk_load(st + C::oSfw + C::kSf, p.ws + (block[1] + i) * 512, 512, b, pol);
         }
       }
-      if (!ok)   // gave up: what this thread still has in flight lands before the CTA may end
-        for (int j = i - 1; j >= 0 && j >= i - C::kStages; j--) bounded_wait(bar(full, j % C::kStages), (j / C::kStages) & 1, abort_flag, p.status, 51, j);
+      // What this thread has in flight lands before the CTA may end (it fills every stage itself: all but the last turns have been seen to land).
+      for (int j = i - 1; j >= 0 && j >= i - C::kStages; j--) wait(bar(full, j % C::kStages), (j / C::kStages) & 1, 51, j);
     }
   } else if (warp == kWarpMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm + C::oTmem), "n"(C::kCols) : "memory");
@@ -544,7 +554,12 @@ __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const _
           mma_bs(tmem, a + (uint64_t)(kb * 2), b + (uint64_t)(kb * 2), instr_desc_bs(128, 256, 0, 5, kb, kb), sf, sf + 4, (i || kb) ? 1u : 0u);
         if (i + C::kStages < nk) tc_commit(bar(C::oBarE, s));   // (nobody waits for the last ones)
       }
-      if (ok) tc_commit(bar(C::oBarDone, 0));
+      if (ok) {
+        tc_commit(bar(C::oBarDone, 0));
+      } else if (tmem != kNoTmem) {   // gave up: what has been issued ends before tensor memory goes back
+        tc_commit(bar(C::oBarLast, 0));
+        ended_wait(bar(C::oBarLast, 0), 0);
+      }
     }
   } else {
     // ---- x's scales: thread r has row r's four bytes of every step, two loads ahead
@@ -729,7 +744,7 @@ size_t uq_fp4_linear_scratch(long long M, int K) { return M <= tc::kDirectRows |
 // xs null: x is bf16 [M, K], scratch holds uq_fp4_linear_scratch bytes; else x is e4m3 [M, K] with scale bytes xs [M, K / 32].
 // launches: kernels enqueued.
 cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, void* out, void* scratch, long long M, int N, int K, int out_dtype,
-                                   unsigned int* status, int sms, bool expire, cudaStream_t s, int* launches) {
+                                   unsigned int* status, int sms, int expire, cudaStream_t s, int* launches) {
   *launches = 0;
   if (M < 0 || M > (1 << 24) || N < 1 || N > (1 << 24) || K < 32 || K > (1 << 24) || K % 32 || out_dtype < 0 || out_dtype > 2) return cudaErrorInvalidValue;
   if (M == 0) return cudaSuccess;

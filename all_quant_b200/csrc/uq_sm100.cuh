@@ -182,6 +182,13 @@ static __device__ __noinline__ bool bounded_wait(uint32_t bar, uint32_t parity, 
     }
   }
 }
+// The same for what comes by itself whatever becomes of the call (copies and instructions in flight, another CTA's pushes): no abort flag ends it, and its
+// limit, in tries and in time, is far above what the others' limited waits can take (a second, then 64 tries each).
+static __device__ __noinline__ void ended_wait(uint32_t bar, uint32_t parity) {
+  const unsigned long long t_start = now_ns();
+  for (unsigned it = 1; !mbar_try(bar, parity); it++)
+    if (it > 20000u && now_ns() - t_start > 20000000000ull) return;
+}
 
 // ---------------------------------------------------------------------------------------------- host
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,

@@ -797,3 +797,39 @@ for B in (4083, 4084, 4085, 4090, 4095, 4096, 16384):
     assert int(taken) == new.sum() and (slots.cpu().numpy() == page * 16 + (lens - 1) % 16).all(), B
 """
     subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT, timeout=300)
+
+
+def test_no_cta_of_the_products_ends_before_what_is_sent_to_it_or_issued_by_it():
+    """The order that keeps a push from reaching a CTA that has ended, and a copy or an instruction from outliving its CTA, on the paths that give up too
+    (read from the source: on a GPU the wrong order is a fault)."""
+    from tests.test_kernel_order import kernels
+    bodies = kernels("uq_linear.cu")
+    body = bodies["uq_fp4_linear_kernel"]
+    # behind the last barrier of a CTA in which anybody gave up: its pushes are waited for, with nothing that cuts the wait short
+    assert body.rindex("__syncthreads();") < body.index("} else if (*abort_flag) {") < body.index("ended_wait(bar(C::oBarIn, 0), 0);")
+    assert body.count("return;") == 1 and body.index("return;") < body.index("mbar_init")
+    for body in bodies.values():
+        # the copying threads see their copies land, the issuing thread its instructions end, whoever gave up
+        assert body.rindex("bulk_load(") < body.rindex(", 51, j)" if ", 51, j)" in body else ", 41, j)") and "bounded_wait(" not in body.replace("if (!r) r = bounded_wait(", "")
+        assert body.index("tc_commit(bar(C::oBarLast, 0));") < body.index("ended_wait(bar(C::oBarLast, 0), 0);") < body.index("tcgen05.dealloc")
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K,bf16", [(3, 256, 1024, True), (8, 256, 1024, True), (20, 256, 2048, False), (64, 300, 1024, True)])
+def test_one_cta_of_a_cluster_gives_up(M, N, K, bf16, monkeypatch):
+    """UQ_B200_CFG=expire=43: only the last CTA of every cluster misses an arrival.  The others have pushed their partials long before it gives up, wait
+    for its pushes, and stay until they have come: NaN everywhere, a record, and the next call is right."""
+    wc, ws = _weight(N, K, 8)
+    x = _rand((M, K), torch.bfloat16, 8)
+    codes, scales, _ = uq_cuda.rms_norm_mx8(x)
+    call = (lambda: uq_cuda.fp4_linear(x, wc, ws, N)) if bf16 else (lambda: uq_cuda.fp4_linear(codes, wc, ws, N, scales=scales))
+    want = call()
+    assert uq_cuda.last_status() == (0, 0, 0, 0) and not want.isnan().any()
+    monkeypatch.setenv("UQ_B200_CFG", "expire=43")
+    assert call().isnan().all()
+    st = uq_cuda.last_status()
+    assert st[0] == 1 and 40 <= st[2] < 60, st
+    monkeypatch.delenv("UQ_B200_CFG")
+    for _ in range(2):
+        assert torch.equal(call(), want)
+        assert uq_cuda.last_status() == (0, 0, 0, 0)
