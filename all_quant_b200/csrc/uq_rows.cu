@@ -57,6 +57,9 @@ UQ_DEV float inverse_root(float v) {   // (v is never subnormal: eps is not); a 
   return v < 3e38f ? fmaf(0.5f * r, e, r) : r;   // (infinity and NaN as they are)
 }
 
+// Rows whose reciprocal root is above this (entries of 2^-12 and less, with an eps below 2^-24) are scaled up first.
+constexpr float kTinyRow = 4096.f;
+
 // A row per block, or (kOneWarp) per warp; V pieces per lane, the row stays in registers between its two uses.
 // With t = s * w, y = t * inv and amax(y) = amax(t) * inv (a product by one factor keeps the order), so that a value costs one
 // multiplication by inv * 2^-E on its way to its code, a power of two times what y itself rounds to.
@@ -121,6 +124,15 @@ __global__ void __launch_bounds__(kOneWarp ? 128 : 1024) uq_rms_norm_kernel(Norm
       total = row_sum<kOneWarp>(sq0, sums);
       inv = inverse_root(total * a.inv_h);
     }
+    if (inv > kTinyRow) {   // the row is brought near one, so that neither s * w nor inv * 2^-E leaves fp32: by a power of two, which changes no rounding
+      const float up = __uint_as_float(__float_as_uint(inv) & 0x7f800000u);   // (inv is at most 2^63, a row's entries at most sqrt(H) / inv)
+      inv *= __uint_as_float(0x7f000000u - __float_as_uint(up));   // 1 / up
+#pragma unroll
+      for (int i = 0; i < V; i++)
+        if (t + i * lanes < pieces)
+#pragma unroll
+          for (int j = 0; j < kPiece; j++) s[i][j] *= up;
+    }
     uint8_t *pc = a.codes + row * a.H, *ps = a.scales + row * (a.H / kGroup);
 #pragma unroll
     for (int i = 0; i < V; i++) {
@@ -138,7 +150,7 @@ __global__ void __launch_bounds__(kOneWarp ? 128 : 1024) uq_rms_norm_kernel(Norm
       if (in) {
         const uint32_t byte = scale_byte(amax);
         float f = inv * inverse_scale(byte);
-        if (byte < 32u) {   // y below 2^-86: inv * 2^-E may leave fp32, so one after the other
+        if (byte < 32u) {   // y below 2^-86: inv * 2^-E may leave fp32 (from 32 on it is at most 2^12 * 2^95), so one after the other
           f = inverse_scale(byte);
 #pragma unroll
           for (int j = 0; j < kPiece; j++) s[i][j] *= inv;

@@ -833,3 +833,28 @@ def test_one_cta_of_a_cluster_gives_up(M, N, K, bf16, monkeypatch):
     for _ in range(2):
         assert torch.equal(call(), want)
         assert uq_cuda.last_status() == (0, 0, 0, 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("H", [64, 2048, 8192])
+@pytest.mark.parametrize("eps", [2.0 ** -126, 2.0 ** -100, 2.0 ** -70, 1e-12])
+def test_norm_of_tiny_rows(dtype, H, eps):
+    """The smallest eps that is served and rows far below its root: a reciprocal root of up to 2^63, on values whose own products with a weight leave
+    fp32's normal range.  (Nothing is added to the tolerance: a row is multiplied by powers of two only.)"""
+    dt = DT[dtype]
+    size = torch.tensor([2.0 ** -120, 2.0 ** -125, 2.0 ** -100, 2.0 ** -64, 2.0 ** -40, 2.0 ** -13, 0.0], device="cuda")
+    x = (_rand((7, H), torch.float32, 3) * size[:, None]).to(dt)
+    x[:, ::3] = 0
+    x[2, 32:] *= 2.0 ** -20   # a group far above the others
+    w = _rand((H,), torch.float32, 4)
+    w[:32] *= 2.0 ** -24
+    w = w.to(dt)
+    x64, w64 = _f64(x), _f64(w)
+    r = 1 / np.sqrt((x64 ** 2).mean(-1, keepdims=True) + float(np.float32(eps)))
+    check_mx8(*uq_cuda.rms_norm_mx8(x, w, eps=eps)[:2], x64 * r * w64)
+    check_mx8(*uq_cuda.rms_norm_mx8(x, eps=eps)[:2], x64 * r)
+    codes, scales, s = uq_cuda.rms_norm_mx8(x, w, x, eps=eps)   # (the sum's doubling is exact, or zero)
+    r = 1 / np.sqrt(((2 * x64) ** 2).mean(-1, keepdims=True) + float(np.float32(eps)))
+    check_mx8(codes, scales, 2 * x64 * r * w64)
+    assert (_f64(s) == 2 * x64).all()
