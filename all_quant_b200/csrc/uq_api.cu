@@ -304,6 +304,8 @@ int uqb_cache_from_upstream_launch(const uint8_t* slots_in, uint8_t* kc, uint8_t
   return (int)e;
 }
 
+unsigned long long uqb_header_id(void) { return UQB_HEADER_ID; }
+
 // ---- the operators around a layer's attention --------------------------------------------------------------------
 int uqb_plan_step_launch(const int32_t* seq_lens, const int32_t* starts, int K, int32_t* block_table, long long row_stride, const int32_t* free_pages, long long n_free,
                          int64_t* slots, int32_t* taken, int B, long long T, int PAGE, int max_pages, void* stream) {

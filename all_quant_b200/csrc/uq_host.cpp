@@ -3,7 +3,8 @@
 //
 // A decode step calls these several times per layer for 2.5 to 6 us of GPU work each; from Python a call cost the host 11 to 15 us
 // (an allocation 1.4 to 2.4 us, twenty attribute reads and comparisons 3 to 5, the launch through ctypes 3).  The entry points
-// come from the library that uq_cuda.lib() has loaded (`bind`), so that both always are of the same build.
+// come from the library that uq_cuda.lib() has loaded (`bind`), as the types that uq_b200.h gives them; a library built from another text of that
+// header is refused.
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -12,8 +13,11 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <cstdint>
+
+#include "uq_b200.h"
 
 namespace {
 
@@ -21,11 +25,11 @@ using at::Tensor;
 using std::optional;
 typedef long long ll;
 
-int (*plan_fn)(const int32_t*, const int32_t*, int, int32_t*, ll, const int32_t*, ll, int64_t*, int32_t*, int, ll, int, int, void*) = nullptr;
-int (*norm_fn)(const void*, const void*, const void*, void*, uint8_t*, uint8_t*, ll, int, int, float, void*) = nullptr;
-int (*silu_fn)(const void*, uint8_t*, uint8_t*, ll, int, int, void*) = nullptr;
-size_t (*scratch_fn)(ll, int) = nullptr;
-int (*linear_fn)(const void*, const uint8_t*, const uint8_t*, const uint8_t*, void*, void*, ll, int, int, int, void*) = nullptr;
+decltype(&uqb_plan_step_launch) plan_fn = nullptr;
+decltype(&uqb_rms_norm_mx8_launch) norm_fn = nullptr;
+decltype(&uqb_silu_mul_mx8_launch) silu_fn = nullptr;
+decltype(&uqb_fp4_linear_scratch_bytes) scratch_fn = nullptr;
+decltype(&uqb_fp4_linear_launch) linear_fn = nullptr;
 
 #define REFUSE(cond, ...) TORCH_CHECK(!(cond), __VA_ARGS__)
 
@@ -245,16 +249,17 @@ PyObject* fp4_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of the five entry points)
+// bind(addresses of the five entry points, and of uqb_header_id)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 5);
-  void* p[5];
-  for (int i = 0; i < 5; i++) {
+  count(n, 6);
+  void* p[6];
+  for (int i = 0; i < 6; i++) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) return nullptr;
     REFUSE(!p[i], "uq_host: an entry point is missing");
   }
+  REFUSE(reinterpret_cast<decltype(&uqb_header_id)>(p[5])() != UQB_HEADER_ID, "uq_host: the library and this module are of different builds: python -m all_quant_b200.build");
   plan_fn = reinterpret_cast<decltype(plan_fn)>(p[0]);
   norm_fn = reinterpret_cast<decltype(norm_fn)>(p[1]);
   silu_fn = reinterpret_cast<decltype(silu_fn)>(p[2]);
@@ -270,4 +275,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_uq_host", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__uq_host() { return PyModule_Create(&module); }
+#ifndef UQ_TORCH_VERSION
+#define UQ_TORCH_VERSION TORCH_VERSION
+#endif
+PyMODINIT_FUNC PyInit__uq_host() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", UQ_TORCH_VERSION) < 0) { Py_DECREF(m); return nullptr; }
+  return m;
+}

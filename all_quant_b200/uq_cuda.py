@@ -42,7 +42,8 @@ EXPORTS = ("uqb_block_m", "uqb_mo_elems", "uqb_ml_elems", "uqb_workspace_bytes",
            "uqb_decode_launch_static", "uqb_static_scratch_bytes",
            "uqb_peer_bytes", "uqb_peer_alloc", "uqb_peer_open", "uqb_peer_close", "uqb_peer_free", "uqb_decode_partial_push_launch", "uqb_merge_wait_launch",
            "uqb_cache_to_upstream_launch", "uqb_cache_from_upstream_launch",
-           "uqb_plan_step_launch", "uqb_rms_norm_mx8_launch", "uqb_silu_mul_mx8_launch", "uqb_fp4_linear_scratch_bytes", "uqb_fp4_linear_launch")
+           "uqb_plan_step_launch", "uqb_rms_norm_mx8_launch", "uqb_silu_mul_mx8_launch", "uqb_fp4_linear_scratch_bytes", "uqb_fp4_linear_launch",
+           "uqb_header_id")
 
 
 def lib():
@@ -70,7 +71,7 @@ def lib():
         L.uqb_tree_decode_launch.argtypes = [pp, vp, vp]
         L.uqb_merge_packed_launch.argtypes = [vp, i, sz, i, vp, vp]
         L.uqb_last_status.argtypes = [ctypes.POINTER(ctypes.c_uint32)]
-        L.uqb_launch_count.restype = ctypes.c_ulonglong
+        L.uqb_launch_count.restype = L.uqb_header_id.restype = ctypes.c_ulonglong
         L.uqb_debug_events.argtypes = [vp, vp]
         L.uqb_debug_events.restype = None
         L.uqb_decode_launch_static.argtypes = [pp, i, i, vp]
@@ -503,7 +504,7 @@ def quantize_on_write(x, code, scale, slots, rule="ceil", c=None, kernel=None):
 # ---- the operators around a layer's attention (not in the reference) -----------------------------------------------
 # Their checks, allocations and launches are in csrc/uq_host.cpp: a decode step calls them several times per layer for 2.5 to 6 us of
 # GPU work each, and the same steps in Python cost the host two to three times that.
-_HOST_FNS = ("uqb_plan_step_launch", "uqb_rms_norm_mx8_launch", "uqb_silu_mul_mx8_launch", "uqb_fp4_linear_scratch_bytes", "uqb_fp4_linear_launch")
+_HOST_FNS = ("uqb_plan_step_launch", "uqb_rms_norm_mx8_launch", "uqb_silu_mul_mx8_launch", "uqb_fp4_linear_scratch_bytes", "uqb_fp4_linear_launch", "uqb_header_id")
 _host_module = None
 
 
@@ -518,6 +519,8 @@ def _host():
         spec = importlib.util.spec_from_file_location("_uq_host", path)
         m = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(m)
+        if m.torch_version != torch.__version__:   # (compiled against torch's C++ headers)
+            raise RuntimeError(f"{path} was built for torch {m.torch_version}, this is {torch.__version__}: run `python -m all_quant_b200.build`")
         m.bind(*(ctypes.cast(getattr(lib(), f), ctypes.c_void_p).value for f in _HOST_FNS))
         _host_module = m
     return _host_module

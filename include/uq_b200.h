@@ -232,6 +232,12 @@ int uqb_last_path(void);
 void uqb_debug_events(void* before, void* after);
 /* Kernels launched by this library in this process (all threads). */
 unsigned long long uqb_launch_count(void);
+/* Which text of this header the library was built from (a digest; 0 where the build gave none): a caller compiled against the header asks
+ * before it relies on the prototypes above. */
+unsigned long long uqb_header_id(void);
+#ifndef UQB_HEADER_ID
+#define UQB_HEADER_ID 0ull
+#endif
 
 #ifdef __cplusplus
 }
