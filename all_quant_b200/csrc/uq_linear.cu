@@ -6,7 +6,8 @@
 // and every 128 x 128 block is 8 KB of codes and 512 bytes of scales, both contiguous.
 // Activations are e4m3 codes with one UE8M0 scale per 32 channels; bf16 rows are split into two such planes, whose products are
 // added: up to 4 rows by the CTAs themselves, on their way into shared memory, more by a kernel of their own first (uq_rows.cu), so
-// that not every tile of the weight does it again.
+// that not every tile of the weight does it again.  A group of wide range, of which two planes would leave out too
+// much (mx8::wide_group), takes four: each 128 channels that hold one get two steps of their own, behind the others (ExtraSteps).
 //
 // What bounds it: reading the weight, N * K * 17 / 32 bytes, up to about 128 rows; so nothing is decoded by threads.  The block-scaled
 // tensor instruction (kind::mxf8f6f4, one UE8M0 scale per 32 elements of K) takes the weight's codes and scale bytes as they are,
@@ -52,7 +53,7 @@ constexpr uint32_t kNoTmem = 0xffffffffu;   // no address of tensor memory
 
 struct LinearParams {
   const uint8_t* xs;    // [rows of the x map, K / 32]
-  const __nv_bfloat16* x16;   // [M, K] rows that the CTAs split themselves
+  const __nv_bfloat16* x16;   // [M, K] bf16 rows: those that the CTAs split themselves, or those that the planes were made of
   const uint8_t* wc;
   const uint8_t* ws;
   void* out;
@@ -63,6 +64,69 @@ struct LinearParams {
   int words;            // x's scale bytes of 128 channels are aligned words
   int pdl;
   int expire;           // for the test of the give-up path: the first step's scales of x are never announced (1: by any CTA, 2: by the last of each cluster)
+};
+
+// Steps behind a CTA's nk own: two for each of them in which a row has a group of wide range (marked by kWideByte, its planes are zeros), for that group's
+// two planes and for the planes of what those leave out.  A bit per step in shared memory, or per run of steps where they are more than the bits; set
+// while x's scales are brought, read once they all are (oBarMap), in ascending order: sums stay the same whoever came first.
+struct ExtraSteps {
+  static constexpr int kWords = 32, kBytes = 4 * kWords + 4;
+  uint32_t at;   // of the words, and of one more that says whether there is a bit at all
+  int nk, shift;
+  UQ_DEV ExtraSteps(uint32_t at_, int nk_) : at(at_), nk(nk_), shift(0) {
+    while ((nk - 1) >> shift >= 32 * kWords) shift++;
+  }
+  UQ_DEV uint32_t word(int w) const {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at + 4 * w) : "memory");
+    return v;
+  }
+  UQ_DEV bool any() const { return __builtin_expect(word(kWords) != 0u, 0); }
+  UQ_DEV int bit(int i) const { return i >> shift; }
+  UQ_DEV void mark(int w, uint32_t bits) const {
+    asm volatile("red.shared.or.b32 [%0], %1;" ::"r"(at + 4 * w), "r"(bits) : "memory");
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 4 * kWords), "r"(1) : "memory");
+  }
+  // f(i, k), until it says no: steps i and i + 1, from nk on, are for step k's channels
+  template <typename F>
+  UQ_DEV void each(F f) const {
+    int i = nk;
+    for (int w = 0; w <= (nk - 1) >> shift >> 5; w++)
+      for (uint32_t m = word(w); m; m &= m - 1) {
+        const int first = (32 * w + __ffs(m) - 1) << shift;
+        for (int k = first; k < min(nk, first + (1 << shift)); k++, i += 2)
+          if (!f(i, k)) return;
+      }
+  }
+};
+
+UQ_DEV void rows_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }   // of the first four warps
+UQ_DEV bool wait_bar(uint32_t b, uint32_t parity, volatile int* abort_flag, unsigned int* status, int id, int k) {
+  bool r = mbar_test(b, parity);
+  if (!r) r = mbar_try(b, parity);
+  if (!r) r = bounded_wait(b, parity, abort_flag, status, id, k);
+  return r;
+}
+
+// One thread's marks: it takes the scale words of a row as they come and looks for kWideByte.
+struct Marks {
+  const ExtraSteps& extra;
+  int word;
+  uint32_t bits = 0;
+  UQ_DEV Marks(const ExtraSteps& e, int i) : extra(e), word(e.bit(i) >> 5) {}
+  UQ_DEV void flush() {
+    if (bits) extra.mark(word, bits);
+    bits = 0;
+  }
+  UQ_DEV void step(int i, uint32_t w) {
+    const int b = extra.bit(i);
+    if (b >> 5 != word) {
+      flush();
+      word = b >> 5;
+    }
+    static_assert(mx8::kWideByte == 0, "a zero byte, found by its borrow");
+    if ((w - 0x01010101u) & ~w & 0x80808080u) bits |= 1u << (b & 31);
+  }
 };
 
 template <int NB, int PLANES>
@@ -80,8 +144,8 @@ struct LinCfg {
   static constexpr int oP = kBeside ? kRing : 0;
   static constexpr int kBody = oP + kP > kRing ? oP + kP : kRing;
   static constexpr int oBarIn = kBody, oBarTmem = oBarIn + 8, oBarDone = oBarTmem + 8, oBarF = oBarDone + 8, oBarE = oBarF + 8 * kStages;
-  static constexpr int oBarLast = oBarE + 8 * kStages, oTmem = oBarLast + 8, oAbort = oTmem + 4;
-  static constexpr int kSmem = oAbort + 4;
+  static constexpr int oBarLast = oBarE + 8 * kStages, oBarDone2 = oBarLast + 8, oBarMap = oBarDone2 + 8, oTmem = oBarMap + 8, oAbort = oTmem + 4, oExtra = oAbort + 4;
+  static constexpr int kSmem = oExtra + ExtraSteps::kBytes;
   static constexpr int cSf = NB;                             // first column of the scales: 8 per stage (4 of the weight, 4 of x)
   static constexpr int kColsUsed = cSf + 8 * kStages;
   static constexpr int kCols = kColsUsed <= 64 ? 64 : (kColsUsed <= 128 ? 128 : 256);   // two CTAs' share an SM's 512
@@ -134,6 +198,151 @@ UQ_DEV void store4(T* o, const float* v, int n, int N) {
   }
 }
 
+// (for the CTAs that split x: what seldom runs stays out of their loop)
+static __device__ __noinline__ bool wide_group_far(uint4 raw, uint2 hi, uint2 lo, uint32_t hi_byte, uint32_t lo_byte) { return mx8::wide_group(raw, hi, lo, hi_byte, lo_byte); }
+
+// x for a pair of extra steps, into the operands t0, t1 and their scales s0, s1: 128 channels (step k) of the tile's rows, the planes of wide groups into
+// rows r and ROWS + r, zeros for all other groups (a row's sums do not depend on its neighbours).  A warp of WARPS has ROWS / WARPS rows and takes a group
+// at a time, a channel per lane: few registers, which all launches of these kernels pay for (with eight channels per lane the kernel had 91 of them instead
+// of 56, and 8 rows x 10240 x 8192, two CTAs per SM, took 13.8 us instead of 13.3).
+template <int ROWS, int WARPS, bool kDirect>
+UQ_DEV void extra_rows(const LinearParams& p, int m0, int rows, int k, int warp, uint8_t* t0, uint8_t* t1, uint8_t* s0, uint8_t* s1) {
+  constexpr int n = ROWS / WARPS;
+  const int lane = threadIdx.x & 31, r0 = warp * n;
+  for (int i = lane; i < 8 * n; i += 32) {
+    const int at = (r0 + i / 8) * 128 + i % 8 * 16;
+    *reinterpret_cast<uint4*>(t0 + at) = *reinterpret_cast<uint4*>(t0 + ROWS * 128 + at) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(t1 + at) = *reinterpret_cast<uint4*>(t1 + ROWS * 128 + at) = make_uint4(0, 0, 0, 0);
+  }
+  auto scales_of = [](int r) { return (r & 31) * 16 + (r >> 5) * 4; };
+  uint32_t groups = 0;   // of row r0 + lane
+  if (lane < n) {
+    const int r = r0 + lane;
+    *reinterpret_cast<uint32_t*>(s0 + scales_of(r)) = *reinterpret_cast<uint32_t*>(s0 + scales_of(ROWS + r)) = 0x01010101u;
+    *reinterpret_cast<uint32_t*>(s1 + scales_of(r)) = *reinterpret_cast<uint32_t*>(s1 + scales_of(ROWS + r)) = 0x01010101u;
+    if (r < rows)
+      for (int g = 0; g < 4 && 4 * k + g < p.K / 32; g++)
+        if (kDirect || p.xs[(long long)(2 * m0 + r) * (p.K / 32) + 4 * k + g] == mx8::kWideByte) groups |= 1u << g;   // (m0: a multiple of ROWS)
+  }
+  __syncwarp();
+  int r = -1;
+  uint32_t left = 0;
+  auto next = [&]() -> int {   // the next group, its row in r; -1: no more
+    while (!left) {
+      if (++r >= n) return -1;
+      left = __shfl_sync(0xffffffffu, groups, r);
+    }
+    const int g = __ffs(left) - 1;
+    left &= left - 1;
+    return g;
+  };
+  auto load = [&](int g) -> uint32_t { return *reinterpret_cast<const unsigned short*>(p.x16 + (long long)(m0 + r0 + r) * p.K + 128 * k + 32 * g + lane); };
+  int g = next();
+  uint32_t x = g < 0 ? 0u : load(g);
+#pragma unroll 1
+  while (g >= 0) {
+    const int row = r0 + r, c = 32 * g + lane;
+    const uint32_t bits = x & 0x7fffu;
+    float v = __uint_as_float(x << 16);
+    uint8_t* at0 = t0 + row * 128 + (((c >> 4) ^ (row & 7)) << 4) + (c & 15);
+    const int to1 = (int)(t1 - t0), sf = scales_of(row) + g, sf2 = scales_of(ROWS + row) + g;
+    g = next();
+    if (g >= 0) x = load(g);
+    if (kDirect && __any_sync(0xffffffffu, bits >= 0x7f80u)) continue;
+    uint32_t codes = 0;   // four planes' and their bytes
+    uint32_t bytes = 0;
+    bool wide = true;
+#pragma unroll 1
+    for (int i = 0; i < 32; i += 8) {
+      const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v))));
+      if (kDirect && i == 16) wide = mx8::wide_rule(__reduce_add_sync(0xffffffffu, bits), __popc(__ballot_sync(0xffffffffu, bits != 0)), amax);
+      const uint32_t byte = max(mx8::scale_byte(amax), 1u), code = mx8::e4m3x2(__fmul_rn(v, mx8::inverse_scale(byte)), 0.f) & 0xffu;
+      v = fmaf(mx8::e4m3_value(code), -uq_scale_f32(byte), v);
+      codes |= code << i;
+      bytes |= byte << i;
+    }
+    if (!wide) continue;
+    at0[0] = (uint8_t)codes;
+    at0[ROWS * 128] = (uint8_t)(codes >> 8);
+    at0[to1] = (uint8_t)(codes >> 16);
+    at0[to1 + ROWS * 128] = (uint8_t)(codes >> 24);
+    if (lane == 0) {
+      s0[sf] = (uint8_t)bytes;
+      s0[sf2] = (uint8_t)(bytes >> 8);
+      s1[sf] = (uint8_t)(bytes >> 16);
+      s1[sf2] = (uint8_t)(bytes >> 24);
+    }
+  }
+}
+
+// The extra steps of the kernel below, for its first four warps, which bring them whole, and for its issuing thread.
+template <typename C, int kScaleWarps, bool kDirect>
+__device__ __noinline__ bool bring_extra(const LinearParams& p, const CUtensorMap& map_w, uint32_t sm, uint8_t* smem, int nk, int k0, int tile_n, int m0, int rows) {
+  constexpr int kGroups = 4 / kScaleWarps;
+  const int warp = threadIdx.x >> 5;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::oAbort);
+  bool ok = true;
+  int issued = nk;
+  auto free_stage = [&](int i) -> bool {
+    const int s = i % C::kStages;
+    return ok = __all_sync(0xffffffffu, i < C::kStages || wait_bar(sm + C::oBarE + 8 * s, ((i / C::kStages) & 1) ^ 1, abort_flag, p.status, 45, i));
+  };
+  ExtraSteps(sm + C::oExtra, nk).each([&](int i, int k) -> bool {
+    const int mine = i + ((i ^ warp) & 1);   // two warps take turns at the weight's codes, two at its scales
+    if (!free_stage(mine)) return false;
+    if (elect_one()) {
+      const uint32_t st = sm + mine % C::kStages * C::kStage, b = sm + C::oBarF + 8 * (mine % C::kStages);
+      const size_t block = (size_t)tile_n * p.ksteps + k0 + k;
+      mbar_expect_tx(b, warp < 2 ? 8192 : C::kSf);
+      if (warp < 2) tma_load_4d(st, &map_w, 0, 0, 0, (int)block, b, l2_policy());
+      else bulk_load(st + C::oSfa, p.ws + block * 512, 512, b, l2_policy());
+      issued = mine + 1;
+    }
+    __syncwarp();
+    if (((i - nk) >> 1) % kGroups == warp / kScaleWarps) {
+      if (!free_stage(i) || !free_stage(i + 1)) return false;
+      uint8_t *st0 = smem + i % C::kStages * C::kStage, *st1 = smem + (i + 1) % C::kStages * C::kStage;
+      extra_rows<C::kRows, kScaleWarps, kDirect>(p, m0, rows, k0 + k, warp % kScaleWarps, st0 + C::oB, st1 + C::oB, st0 + C::oSfb, st1 + C::oSfb);
+      fence_async_smem();
+      __syncwarp();
+      if ((threadIdx.x & 31) < 2) mbar_arrive(sm + C::oBarF + 8 * ((i + (threadIdx.x & 31)) % C::kStages));
+    }
+    return true;
+  });
+  ok = __all_sync(0xffffffffu, ok && wait_bar(sm + C::oBarDone2, 0, abort_flag, p.status, 46, nk));
+  if (!ok)   // gave up: what this thread has copied lands before the CTA may end (where such a stage has been filled again, the wait runs out)
+    for (int j = issued - 1; j >= nk && j >= issued - 2 * C::kStages; j -= 2) wait_bar(sm + C::oBarF + 8 * (j % C::kStages), (j / C::kStages) & 1, abort_flag, p.status, 41, j);
+  __syncwarp();
+  return ok;
+}
+template <typename C, int NB>
+UQ_DEV void multiply_step(uint32_t sm, uint32_t tmem, int s, bool first) {
+  tc_fence_after();
+  const uint32_t st = sm + s * C::kStage, sf = tmem + C::cSf + 8 * s;
+  tmem_copy_sf(sf, sf_desc(st + C::oSfa));
+  tmem_copy_sf(sf + 4, sf_desc(st + C::oSfb));
+  const uint64_t a = smem_desc(st, 16, 1024), b = smem_desc(st + C::oB, 16, 1024);
+#pragma unroll
+  for (int kb = 0; kb < 4; kb++)
+    mma_bs(tmem, a + (uint64_t)(kb * 2), b + (uint64_t)(kb * 2), instr_desc_bs(128, NB, 5, 0, kb, kb), sf, sf + 4, (!first || kb) ? 1u : 0u);
+}
+template <typename C, int NB>
+__device__ __noinline__ bool multiply_extra(uint32_t sm, volatile int* abort_flag, unsigned int* status, uint32_t tmem, int nk) {
+  bool ok = true;
+  for (int j = max(nk - C::kStages, 0); j < nk; j++) tc_commit(sm + C::oBarE + 8 * (j % C::kStages));   // the last stages of the steps before, which nobody has waited for
+  ExtraSteps(sm + C::oExtra, nk).each([&](int first, int) -> bool {
+    for (int i = first; i < first + 2; i++) {
+      const int s = i % C::kStages;
+      if (!(ok = wait_bar(sm + C::oBarF + 8 * s, (i / C::kStages) & 1, abort_flag, status, 42, i))) return false;
+      multiply_step<C, NB>(sm, tmem, s, false);
+      tc_commit(sm + C::oBarE + 8 * s);
+    }
+    return true;
+  });
+  if (ok) tc_commit(sm + C::oBarDone2);
+  return ok;
+}
+
 template <int NB, int PLANES, bool kDirect>
 __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid_constant__ LinearParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
   using C = LinCfg<NB, PLANES>;
@@ -151,12 +360,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_lin + C::oAbort);
   auto stage_at = [&](int s) { return sm + s * C::kStage; };
   auto bar = [&](int o, int s) { return sm + o + 8 * s; };
-  auto wait = [&](uint32_t b, uint32_t parity, int id, int k) -> bool {
-    bool r = mbar_test(b, parity);
-    if (!r) r = mbar_try(b, parity);
-    if (!r) r = bounded_wait(b, parity, abort_flag, p.status, id, k);
-    return r;
-  };
+  auto wait = [&](uint32_t b, uint32_t parity, int id, int k) -> bool { return wait_bar(b, parity, abort_flag, p.status, id, k); };
   const size_t block0 = (size_t)tile_n * p.ksteps + k0;   // first 128 x 128 block of this CTA's range
   // A step's stage has one barrier for all that comes into it (weight, x with the weight's scales, x's scales): every barrier looked at
   // costs the issuing thread 30 of the 460 cycles that a step took it with three.
@@ -164,7 +368,11 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   // (A wait by parity tells a phase from its neighbours only: the warps of a role that take turns are no more than the stages, so that
   // a warp's step before this one has seen the phase before the one that it now waits for.)
   auto wait_free = [&](int i, int id) -> bool { return i < C::kStages || wait(bar(C::oBarE, i % C::kStages), ((i / C::kStages) & 1) ^ 1, id, i); };
-  constexpr int kScaleWarps = (NB + 31) / 32;
+  constexpr int kScaleWarps = (NB + 31) / 32, kGroups = 4 / kScaleWarps;   // warps that bring a step's scales (or x itself), and how many such groups take turns
+  static_assert(kGroups <= C::kStages && 2 <= C::kStages, "no more turns than stages");
+  constexpr bool kExtra = PLANES == 2;
+  const ExtraSteps extra(sm + C::oExtra, nk);
+  static_assert(ExtraSteps::kWords == 32, "a word per lane");
 
   const long long m0 = (long long)tile_m * C::kRows;
   const int rows = (int)min((long long)C::kRows, p.M - m0);   // of this tile
@@ -172,13 +380,15 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   const bool expire = p.expire == 1 || (p.expire == 2 && rank == split - 1);
 
   if (warp == 0) {   // a barrier per lane
-    constexpr int kBars = 4 + 2 * C::kStages;
+    constexpr int kBars = 6 + 2 * C::kStages;
     static_assert(kBars <= 32 && C::oBarE == C::oBarIn + 8 * (3 + C::kStages), "barriers lie side by side");
-    if (lane < kBars) mbar_init(sm + C::oBarIn + 8 * lane, lane >= 3 && lane < 3 + C::kStages ? 2 + kScaleWarps : 1);
+    if (lane < kBars) mbar_init(sm + C::oBarIn + 8 * lane, lane >= 3 && lane < 3 + C::kStages ? 2 + kScaleWarps : (lane == kBars - 1 ? 4 : 1));
+    if (kExtra) *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oExtra + 4 * lane) = 0;
     fence_barrier_init();
     if (lane == 0) {
       *abort_flag = 0;
       *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem) = kNoTmem;
+      *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oExtra + 4 * ExtraSteps::kWords) = 0;
     }
     __syncwarp();
     if (split > 1 && lane == 0) mbar_expect_tx(bar(C::oBarIn, 0), (uint32_t)(mine * split * C::kPRow));   // (no rows: complete at once)
@@ -193,16 +403,16 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
   int issued = 0;   // by a copying thread: every other step below it
   if (warp >= kWarpW) {
     // ---- copies: two threads each for the weight's codes, and for x with the weight's scales
+    const bool weights = warp < kWarpX;
+    const int turn = weights ? warp - kWarpW : warp - kWarpX;
     if (elect_one()) {
-      const bool weights = warp < kWarpX;
       const uint64_t pol = l2_policy();
       uint64_t keep;
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));   // (x is read by every tile; 4096 x 4096: 5.2 us, 6.0 without)
-      int i = weights ? warp - kWarpW : warp - kWarpX;
+      int i = turn;
       for (; i < nk; i += 2) {
-        const int s = i % C::kStages;
         if (!wait_free(i, 40)) break;
-        const uint32_t st = stage_at(s), b = full_bar(i);
+        const uint32_t st = stage_at(i % C::kStages), b = full_bar(i);
         if (weights) {
           mbar_expect_tx(b, 8192);   // the packed bytes are counted
           tma_load_4d(st, &map_w, 0, 0, 0, (int)(block0 + i), b, pol);
@@ -237,31 +447,24 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         const int s1 = s + 1 == C::kStages ? 0 : s + 1;
         const uint32_t parity1 = parity ^ (s1 == 0 ? 1u : 0u);
         here = mbar_test(bar(C::oBarF, s1), parity1);
-        tc_fence_after();
-        const uint32_t st = stage_at(s), sf = tmem + C::cSf + 8 * s;
-        tmem_copy_sf(sf, sf_desc(st + C::oSfa));
-        tmem_copy_sf(sf + 4, sf_desc(st + C::oSfb));
-        const uint64_t a = smem_desc(st, 16, 1024), b = smem_desc(st + C::oB, 16, 1024);
-#pragma unroll
-        for (int kb = 0; kb < 4; kb++)
-          mma_bs(tmem, a + (uint64_t)(kb * 2), b + (uint64_t)(kb * 2), instr_desc_bs(128, NB, 5, 0, kb, kb), sf, sf + 4, (i || kb) ? 1u : 0u);
-        if (i + C::kStages < nk) tc_commit(bar(C::oBarE, s));   // (nobody waits for the last ones)
+        multiply_step<C, NB>(sm, tmem, s, i == 0);
+        if (i + C::kStages < nk) tc_commit(bar(C::oBarE, s));   // (nobody waits for the last ones, but for the steps behind them)
         s = s1;
         parity = parity1;
       }
-      if (ok) {
-        tc_commit(bar(C::oBarDone, 0));
-      } else if (tmem != kNoTmem) {   // gave up: what has been issued ends before tensor memory goes back
+      if (ok) tc_commit(bar(C::oBarDone, 0));
+      if (kExtra && ok && (ok = wait(bar(C::oBarMap, 0), 0, 44, nk)) && extra.any()) ok = multiply_extra<C, NB>(sm, abort_flag, p.status, tmem, nk);
+      if (!ok && tmem != kNoTmem) {   // gave up: what has been issued ends before tensor memory goes back
         tc_commit(bar(C::oBarLast, 0));
         ended_wait(bar(C::oBarLast, 0), 0);
       }
     }
   } else {
+    int i = warp / kScaleWarps;
     if constexpr (kDirect) {
       // ---- x itself: a warp splits a step's 4 rows x 128 channels (lane: piece lane % 16 of rows lane / 16 and 2 + lane / 16) into the two planes of the
       // tile, rows r and 8 + r of 128 bytes with the 128-byte swizzle, and their scale bytes; the next step's loads are on their way.
       static_assert(!kDirect || (NB == 16 && PLANES == 2), "rows of both planes");
-      static_assert(4 <= C::kStages, "four warps take turns");
       constexpr int kPer = kDirectRows / 2;   // pieces of a lane
       const int piece = lane & 15, r0 = lane >> 4;
       mx8::Raw<__nv_bfloat16> next[kPer];
@@ -275,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         }
       };
       load(warp);
-      for (int i = warp; i < nk; i += 4) {
+      for (; i < nk; i += 4) {
         const int s = i % C::kStages;
         uint2 hi[kPer], lo[kPer];
         uint32_t hi_byte[kPer], lo_byte[kPer];
@@ -285,6 +488,22 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
           float v[8];
           next[j].get(v);
           mx8::split_piece(v, hi[j], lo[j], hi_byte[j], lo_byte[j]);
+        }
+        bool look = false;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) look |= 2 * j + r0 < rows && mx8::may_leave(hi[j]);
+        if (__builtin_expect(__any_sync(0xffffffffu, look), 0)) {   // (a step in ten of normally distributed values; with may_be_wide at once: 4 rows x 4096 x 4096 5.19 us, not 5.05)
+          bool any = false;
+#pragma unroll
+          for (int j = 0; j < kPer; j++) {
+            if (2 * j >= rows) break;
+            if (__any_sync(0xffffffffu, mx8::may_be_wide(hi[j])) && wide_group_far(next[j].a, hi[j], lo[j], hi_byte[j], lo_byte[j])) {
+              hi[j] = lo[j] = make_uint2(0, 0);
+              hi_byte[j] = lo_byte[j] = mx8::kWideByte;
+              any = true;
+            }
+          }
+          if (any) extra.mark(extra.bit(i) >> 5, 1u << (extra.bit(i) & 31));
         }
         load(i + 4);
         if (!__all_sync(0xffffffffu, wait_free(i, 45))) break;
@@ -306,11 +525,9 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
       }
     } else {
       // ---- x's scales: thread r of a group of warps has row r's four bytes of the group's steps, two loads ahead
-      constexpr int kGroups = 4 / kScaleWarps;
-      static_assert(kGroups <= C::kStages && 2 <= C::kStages, "as many warps take turns");
       const int r = (warp % kScaleWarps) * 32 + lane, groups = p.K / 32;
       const long long row = (long long)tile_m * NB + r;
-      const bool have = r < NB && row < p.xrows;
+      const bool have = r < NB && row < p.xrows && (!kExtra || r % C::kRows < rows);   // (what lies behind the last row was never written)
       const uint8_t* src = p.xs + row * groups;
       auto load = [&](int i) -> uint32_t {
         uint32_t w = 0x7f7f7f7fu;
@@ -323,8 +540,8 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         }
         return w;
       };
-      int i = warp / kScaleWarps;
       uint32_t w0 = load(i), w1 = load(i + kGroups);
+      Marks marks(extra, i);
       for (; i < nk; i += kGroups) {
         const int s = i % C::kStages;
         if (!__all_sync(0xffffffffu, wait_free(i, 45))) break;
@@ -332,13 +549,23 @@ __global__ void __launch_bounds__(kThreads, 2) uq_fp4_linear_kernel(const __grid
         fence_async_smem();
         __syncwarp();
         if (lane == 0 && (i > 0 || !expire)) mbar_arrive(full_bar(i));
+        if (kExtra) marks.step(i, w0);
         w0 = w1;
         w1 = load(i + 2 * kGroups);
       }
+      if (kExtra) marks.flush();
+    }
+    bool more = false;
+    if (kExtra) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::oBarMap, 0));
+      rows_barrier();
+      more = extra.any();
     }
     // ---- epilogue, first half: the accumulator's lane 32 j + l is channel 4 l + j of the tile.  A row of a partial tile is four runs of
     // 32 floats, one per warp.  Pushed, row t goes to the CTA of rank t % split, place (t / split, this rank).
-    const bool ok = __all_sync(0xffffffffu, wait(bar(C::oBarDone, 0), 0, 46, nk) && wait(bar(C::oBarTmem, 0), 0, 47, nk));
+    bool ok = __all_sync(0xffffffffu, wait(bar(C::oBarDone, 0), 0, 46, nk) && wait(bar(C::oBarTmem, 0), 0, 47, nk));
+    if (more && ok) ok = bring_extra<C, kScaleWarps, kDirect>(p, map_w, sm, smem_lin, nk, k0, tile_n, (int)m0, rows);
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem);
     if (ok) tc_fence_after();
     if (split > 1) {
@@ -448,11 +675,86 @@ struct WideCfg {
   static constexpr int kRing = kStages * kStage;
   static constexpr int kPRow = 257 * 4;                             // bytes of a row of the result, one per operand row (odd in words: a lane per row writes it)
   static constexpr int oBarDone = kRing, oBarTmem = oBarDone + 8, oBarW = oBarTmem + 8, oBarX = oBarW + 8 * kStages, oBarS = oBarX + 8 * kStages, oBarE = oBarS + 8 * kStages;
-  static constexpr int oBarLast = oBarE + 8 * kStages, oTmem = oBarLast + 8, oAbort = oTmem + 4;
-  static constexpr int kSmem = oAbort + 4;
+  static constexpr int oBarLast = oBarE + 8 * kStages, oBarDone2 = oBarLast + 8, oBarMap = oBarDone2 + 8, oTmem = oBarMap + 8, oAbort = oTmem + 4, oExtra = oAbort + 4;
+  static constexpr int kSmem = oExtra + ExtraSteps::kBytes;
   static constexpr int cSf = 256, kCols = 512;                      // columns of the scales: 12 per stage (4 of x, 8 of the weight)
   static_assert(128 * kPRow <= kRing && cSf + 12 * kStages <= kCols && kSmem + 1024 <= 228 * 1024, "fits an SM");
 };
+
+// Its extra steps, as above: every warp has a role in each.
+template <typename C>
+__device__ __noinline__ bool bring_extra_wide(const LinearParams& p, const CUtensorMap& map_w, uint32_t sm, uint8_t* smem, int nk, int pair, int m0, int rows) {
+  const int role = threadIdx.x >> 5;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::oAbort);
+  bool ok = true;
+  int issued = nk;
+  ExtraSteps(sm + C::oExtra, nk).each([&](int first, int k) -> bool {
+    for (int i = first; i < first + 2; i++) {
+      const int s = i % C::kStages;
+      if (!(ok = __all_sync(0xffffffffu, i < C::kStages || wait_bar(sm + C::oBarE + 8 * s, ((i / C::kStages) & 1) ^ 1, abort_flag, p.status, 55, i)))) return false;
+      if (elect_one()) {
+        const uint32_t st = sm + s * C::kStage, b = sm + (role < 2 ? C::oBarW : C::oBarX) + 8 * s;
+        const size_t block0 = (size_t)(2 * pair) * nk + k, block1 = (size_t)min(2 * pair + 1, p.tiles - 1) * nk + k;
+        if (role == 2) {
+          mbar_arrive(b);
+        } else if (role < 2) {
+          mbar_expect_tx(b, 8192);
+          tma_load_4d(st + role * C::kW, &map_w, 0, 0, 0, (int)(role ? block1 : block0), b, l2_policy());
+        } else {
+          mbar_expect_tx(b, 2 * C::kSf);
+          bulk_load(st + C::oSfw, p.ws + block0 * 512, 512, b, l2_policy());
+          bulk_load(st + C::oSfw + C::kSf, p.ws + block1 * 512, 512, b, l2_policy());
+        }
+        issued = i + 1;
+      }
+      __syncwarp();
+    }
+    uint8_t *st0 = smem + first % C::kStages * C::kStage, *st1 = smem + (first + 1) % C::kStages * C::kStage;
+    extra_rows<C::kRows, 4, false>(p, m0, rows, k, role, st0 + C::oX, st1 + C::oX, st0 + C::oSfx, st1 + C::oSfx);
+    fence_async_smem();
+    __syncwarp();
+    if ((threadIdx.x & 31) < 2) mbar_arrive(sm + C::oBarS + 8 * ((first + (threadIdx.x & 31)) % C::kStages));
+    return true;
+  });
+  ok = __all_sync(0xffffffffu, ok && wait_bar(sm + C::oBarDone2, 0, abort_flag, p.status, 56, nk));
+  if (!ok)
+    for (int j = issued - 1; j >= nk && j >= issued - C::kStages; j--)
+      wait_bar(sm + (role < 2 ? C::oBarW : C::oBarX) + 8 * (j % C::kStages), (j / C::kStages) & 1, abort_flag, p.status, 51, j);
+  __syncwarp();
+  return ok;
+}
+template <typename C>
+UQ_DEV bool multiply_step_wide(uint32_t sm, volatile int* abort_flag, unsigned int* status, uint32_t tmem, int i) {
+  const int s = i % C::kStages;
+  const uint32_t parity = (i / C::kStages) & 1;
+  if (!(wait_bar(sm + C::oBarX + 8 * s, parity, abort_flag, status, 52, i) && wait_bar(sm + C::oBarS + 8 * s, parity, abort_flag, status, 53, i) &&
+        wait_bar(sm + C::oBarW + 8 * s, parity, abort_flag, status, 54, i)))
+    return false;
+  tc_fence_after();
+  const uint32_t st = sm + s * C::kStage, sf = tmem + C::cSf + 12 * s;
+  tmem_copy_sf(sf, sf_desc(st + C::oSfx));
+  tmem_copy_sf(sf + 4, sf_desc(st + C::oSfw));
+  tmem_copy_sf(sf + 8, sf_desc(st + C::oSfw + C::kSf));
+  const uint64_t a = smem_desc(st + C::oX, 16, 1024), b = smem_desc(st, 16, 1024);
+#pragma unroll
+  for (int kb = 0; kb < 4; kb++)
+    mma_bs(tmem, a + (uint64_t)(kb * 2), b + (uint64_t)(kb * 2), instr_desc_bs(128, 256, 0, 5, kb, kb), sf, sf + 4, (i || kb) ? 1u : 0u);
+  return true;
+}
+template <typename C>
+__device__ __noinline__ bool multiply_extra_wide(uint32_t sm, volatile int* abort_flag, unsigned int* status, uint32_t tmem, int nk) {
+  bool ok = true;
+  for (int j = max(nk - C::kStages, 0); j < nk; j++) tc_commit(sm + C::oBarE + 8 * (j % C::kStages));
+  ExtraSteps(sm + C::oExtra, nk).each([&](int first, int) -> bool {
+    for (int i = first; i < first + 2 && ok; i++) {
+      ok = multiply_step_wide<C>(sm, abort_flag, status, tmem, i);
+      if (ok) tc_commit(sm + C::oBarE + 8 * (i % C::kStages));
+    }
+    return ok;
+  });
+  if (ok) tc_commit(sm + C::oBarDone2);
+  return ok;
+}
 
 template <int PLANES>
 __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const __grid_constant__ LinearParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
@@ -471,23 +773,22 @@ __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const _
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_lin + C::oAbort);
   auto stage_at = [&](int s) { return sm + s * C::kStage; };
   auto bar = [&](int o, int s) { return sm + o + 8 * s; };
-  auto wait = [&](uint32_t b, uint32_t parity, int id, int k) -> bool {
-    bool r = mbar_test(b, parity);
-    if (!r) r = mbar_try(b, parity);
-    if (!r) r = bounded_wait(b, parity, abort_flag, p.status, id, k);
-    return r;
-  };
+  auto wait = [&](uint32_t b, uint32_t parity, int id, int k) -> bool { return wait_bar(b, parity, abort_flag, p.status, id, k); };
+  constexpr bool kExtra = PLANES == 2;
+  const ExtraSteps extra(sm + C::oExtra, nk);
   // first blocks of the pair's two tiles (an odd number of tiles: the last one twice, its second copy is never stored)
   const size_t block[2] = {(size_t)(2 * pair) * nk, (size_t)min(2 * pair + 1, p.tiles - 1) * nk};
 
   if (warp == 0) {   // a barrier per lane
-    constexpr int kBars = 3 + 4 * C::kStages;
+    constexpr int kBars = 5 + 4 * C::kStages;
     static_assert(kBars <= 32 && C::oBarE == C::oBarDone + 8 * (2 + 3 * C::kStages), "barriers lie side by side");
-    if (lane < kBars) mbar_init(sm + C::oBarDone + 8 * lane, lane < 2 || lane >= 2 + 3 * C::kStages ? 1 : (lane < 2 + 2 * C::kStages ? 2 : 4));
+    if (lane < kBars) mbar_init(sm + C::oBarDone + 8 * lane, lane == kBars - 1 ? 4 : (lane < 2 || lane >= 2 + 3 * C::kStages ? 1 : (lane < 2 + 2 * C::kStages ? 2 : 4)));
+    if (kExtra) *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oExtra + 4 * lane) = 0;
     fence_barrier_init();
     if (lane == 0) {
       *abort_flag = 0;
       *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem) = kNoTmem;
+      *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oExtra + 4 * ExtraSteps::kWords) = 0;
     }
   } else if (warp >= kWarpW && lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(warp < kWarpX ? &map_w : &map_x) : "memory");   // (launch arguments, not global memory)
@@ -498,8 +799,8 @@ __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const _
 
   if (warp >= kWarpW) {
     // ---- copies: a thread each for the two blocks of the weight, for x, and for the weight's scales
+    const int role = warp - kWarpW;
     if (elect_one()) {
-      const int role = warp - kWarpW;
       const uint64_t pol = l2_policy();
       uint64_t keep;
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
@@ -539,60 +840,61 @@ __global__ void __launch_bounds__(kThreads, 1) uq_fp4_linear_wide_kernel(const _
         uq_report(p.status, 1u, 59u, 0u);
       }
       for (int i = 0; i < nk && ok; i++) {
-        const int s = i % C::kStages;
-        const uint32_t parity = (i / C::kStages) & 1;
-        ok = wait(bar(C::oBarX, s), parity, 52, i) && wait(bar(C::oBarS, s), parity, 53, i) && wait(bar(C::oBarW, s), parity, 54, i);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t st = stage_at(s), sf = tmem + C::cSf + 12 * s;
-        tmem_copy_sf(sf, sf_desc(st + C::oSfx));
-        tmem_copy_sf(sf + 4, sf_desc(st + C::oSfw));
-        tmem_copy_sf(sf + 8, sf_desc(st + C::oSfw + C::kSf));
-        const uint64_t a = smem_desc(st + C::oX, 16, 1024), b = smem_desc(st, 16, 1024);
-#pragma unroll
-        for (int kb = 0; kb < 4; kb++)
-          mma_bs(tmem, a + (uint64_t)(kb * 2), b + (uint64_t)(kb * 2), instr_desc_bs(128, 256, 0, 5, kb, kb), sf, sf + 4, (i || kb) ? 1u : 0u);
-        if (i + C::kStages < nk) tc_commit(bar(C::oBarE, s));   // (nobody waits for the last ones)
+        ok = multiply_step_wide<C>(sm, abort_flag, p.status, tmem, i);
+        if (ok && i + C::kStages < nk) tc_commit(bar(C::oBarE, i % C::kStages));   // (nobody waits for the last ones, but for the steps behind them)
       }
-      if (ok) {
-        tc_commit(bar(C::oBarDone, 0));
-      } else if (tmem != kNoTmem) {   // gave up: what has been issued ends before tensor memory goes back
+      if (ok) tc_commit(bar(C::oBarDone, 0));
+      if (kExtra && ok && (ok = wait(bar(C::oBarMap, 0), 0, 52, nk)) && extra.any()) ok = multiply_extra_wide<C>(sm, abort_flag, p.status, tmem, nk);
+      if (!ok && tmem != kNoTmem) {   // gave up: what has been issued ends before tensor memory goes back
         tc_commit(bar(C::oBarLast, 0));
         ended_wait(bar(C::oBarLast, 0), 0);
       }
     }
   } else {
     // ---- x's scales: thread r has row r's four bytes of every step, two loads ahead
-    {
-      const int groups = p.K / 32;
-      const long long row = (long long)tile_m * 128 + tid;
-      const bool have = row < p.xrows;
-      const uint8_t* src = p.xs + row * groups;
-      auto load = [&](int i) -> uint32_t {
-        uint32_t w = 0x7f7f7f7fu;
-        if (have && i < nk) {
-          const int g = i * 4;
-          if (p.words) return *reinterpret_cast<const uint32_t*>(src + g);
+    const int groups = p.K / 32;
+    const long long row = (long long)tile_m * 128 + tid;
+    const bool have = row < p.xrows && (!kExtra || tid % C::kRows < rows);   // (what lies behind the last row was never written)
+    const uint8_t* src = p.xs + row * groups;
+    auto load = [&](int i) -> uint32_t {
+      uint32_t w = 0x7f7f7f7fu;
+      if (have && i < nk) {
+        const int g = i * 4;
+        if (p.words) return *reinterpret_cast<const uint32_t*>(src + g);
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            if (g + j < groups) w = (w & ~(0xffu << (8 * j))) | ((uint32_t)src[g + j] << (8 * j));
-        }
-        return w;
-      };
-      uint32_t w0 = load(0), w1 = load(1);
-      for (int i = 0; i < nk; i++) {
-        const int s = i % C::kStages;
-        if (i >= C::kStages && !__all_sync(0xffffffffu, wait(bar(C::oBarE, s), ((i / C::kStages) & 1) ^ 1, 55, i))) break;
-        *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfx + lane * 16 + warp * 4) = w0;
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0 && (i > 0 || !p.expire)) mbar_arrive(bar(C::oBarS, s));
-        w0 = w1;
-        w1 = load(i + 2);
+        for (int j = 0; j < 4; j++)
+          if (g + j < groups) w = (w & ~(0xffu << (8 * j))) | ((uint32_t)src[g + j] << (8 * j));
       }
+      return w;
+    };
+    uint32_t w0 = load(0), w1 = load(1);
+    Marks marks(extra, 0);
+    int i = 0;
+    auto free_stage = [&](int i) -> bool {
+      return __all_sync(0xffffffffu, i < C::kStages || wait(bar(C::oBarE, i % C::kStages), ((i / C::kStages) & 1) ^ 1, 55, i));
+    };
+    for (; i < nk; i++) {
+      const int s = i % C::kStages;
+      if (!free_stage(i)) break;
+      *reinterpret_cast<uint32_t*>(smem_lin + s * C::kStage + C::oSfx + lane * 16 + warp * 4) = w0;
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0 && (i > 0 || !p.expire)) mbar_arrive(bar(C::oBarS, s));
+      if (kExtra) marks.step(i, w0);
+      w0 = w1;
+      w1 = load(i + 2);
+    }
+    bool more = false;
+    if (kExtra) {
+      marks.flush();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::oBarMap, 0));
+      rows_barrier();
+      more = extra.any();
     }
     // ---- epilogue, first half: lane = row of the operand, column = channel (in the order of the tensor map)
-    const bool ok = __all_sync(0xffffffffu, wait(bar(C::oBarDone, 0), 0, 56, nk) && wait(bar(C::oBarTmem, 0), 0, 57, nk));
+    bool ok = __all_sync(0xffffffffu, wait(bar(C::oBarDone, 0), 0, 56, nk) && wait(bar(C::oBarTmem, 0), 0, 57, nk));
+    if (more && ok) ok = bring_extra_wide<C>(p, map_w, sm, smem_lin, nk, pair, (int)m0, rows);
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_lin + C::oTmem) + ((uint32_t)(warp * 32) << 16);
     if (ok) {
       tc_fence_after();
@@ -761,8 +1063,8 @@ cudaError_t uq_fp4_linear_dispatch(const void* x, const uint8_t* xs, const uint8
   const uint8_t* codes = static_cast<const uint8_t*>(x);
   p.xs = xs;
   p.xrows = M;
+  if (!xs) p.x16 = static_cast<const __nv_bfloat16*>(x);
   if (direct) {
-    p.x16 = static_cast<const __nv_bfloat16*>(x);
     codes = nullptr;
   } else if (planes == 2) {
     p.xrows = plane_rows(M);

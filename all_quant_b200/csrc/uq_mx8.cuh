@@ -117,22 +117,78 @@ UQ_DEV void e4m3x2_to_f32(uint32_t v, float& lo, float& hi) {
   lo = __half2float(__ushort_as_half((unsigned short)(h2 & 0xFFFFu)));
   hi = __half2float(__ushort_as_half((unsigned short)(h2 >> 16)));
 }
-// A piece v into the leading plane's and the remainder's codes and scale bytes (v is used up).
-UQ_DEV void split_piece(float* v, uint2& hi, uint2& lo, uint32_t& hi_byte, uint32_t& lo_byte) {
-  float amax = group_amax(piece_amax(v));
-  hi_byte = scale_byte(amax);
-  hi = codes_of(v, inverse_scale(hi_byte), amax);
-  const float scale = -uq_scale_f32(hi_byte);
-  const uint32_t h[4] = {hi.x & 0xffffu, hi.x >> 16, hi.y & 0xffffu, hi.y >> 16};
+// A piece v into a plane's codes and scale byte, which is at least 1 (zeros too; 2^-126 has the steps that a bf16's last bit needs, and 0 has another use).
+UQ_DEV void plane_of(const float* v, uint2& codes, uint32_t& byte) {
+  const float amax = group_amax(piece_amax(v));
+  byte = max(scale_byte(amax), 1u);
+  codes = codes_of(v, inverse_scale(byte), amax);
+}
+// What a plane leaves out of its piece, exactly: both are multiples of the value's last bit or of the plane's last step, and close together.
+UQ_DEV void take_out(float* v, uint2 codes, uint32_t byte) {
+  const float scale = -uq_scale_f32(byte);
+  const uint32_t h[4] = {codes.x & 0xffffu, codes.x >> 16, codes.y & 0xffffu, codes.y >> 16};
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     float a, b;
     e4m3x2_to_f32(h[i], a, b);
-    fma2(v[2 * i], v[2 * i + 1], a, b, scale, scale, v[2 * i], v[2 * i + 1]);   // exact: both are multiples of x's last bit, at most 8 bits apart
+    fma2(v[2 * i], v[2 * i + 1], a, b, scale, scale, v[2 * i], v[2 * i + 1]);
   }
-  amax = group_amax(piece_amax(v));
-  lo_byte = scale_byte(amax);
-  lo = codes_of(v, inverse_scale(lo_byte), amax);
+}
+// A piece into the leading plane and the remainder's (v is that remainder then).
+UQ_DEV void split_piece(float* v, uint2& hi, uint2& lo, uint32_t& hi_byte, uint32_t& lo_byte) {
+  plane_of(v, hi, hi_byte);
+  take_out(v, hi, hi_byte);
+  plane_of(v, lo, lo_byte);
+}
+// ---- groups of wide range ---------------------------------------------------------------------------------------------
+// What two planes leave out of bf16 values lies under 2^-21 of the group's largest, in values below 2^-13 of it.  Where that is an ordinary group's smallest
+// value it is nothing beside the others.  In a group of wide range - a few large channels, whose codes in the weight may be zero - it is not: the group is
+// "wide" where a value loses more than 2^-14 of the group's typical magnitude, the geometric mean of the values that are not zero (a bf16's bits, read
+// as a whole number, are its logarithm but for the mantissa's curve; no large channel moves that mean far).  All of it is whole numbers and maxima: any
+// order of the lanes gives the same answer.  (Normal or Laplace distributed values, or products of two such: not one group of 131 072.  32 values of which
+// 1, 4 or 8 are 1000 times the others: 17 to 29 %, 16 384 times: 86 to 99.7 %.)
+constexpr uint32_t kWideByte = 0;   // in place of such a group's scales, with codes of zero
+UQ_DEV bool wide_rule(uint32_t sum, uint32_t count, float left) { return left > 6.103515625e-05f * __uint_as_float(sum / max(count, 1u) << 16); }
+
+// Whether a lane's group is wide: its piece with its codes and bytes (not for a group with NaN or infinity, whose own codes say it).
+UQ_DEV bool wide_group(uint4 raw, uint2 hi, uint2 lo, uint32_t hi_byte, uint32_t lo_byte) {
+  Raw<__nv_bfloat16> x;
+  x.a = raw;
+  float rest[kPiece];
+  x.get(rest);
+  take_out(rest, hi, hi_byte);
+  take_out(rest, lo, lo_byte);
+  const float left = group_amax(piece_amax(rest));
+  const uint32_t w[4] = {raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu, raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu};
+  uint32_t n = 0;   // sum of the logarithms, and from bit 24 on how many
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t a = w[i] & 0xffffu, b = w[i] >> 16;
+    n += a + b + (a ? 1u << 24 : 0u) + (b ? 1u << 24 : 0u);
+    finite &= max(a, b) < 0x7f80u;
+  }
+  n += __shfl_xor_sync(0xffffffffu, n, 1);
+  n += __shfl_xor_sync(0xffffffffu, n, 2);
+  const uint32_t others = __ballot_sync(0xffffffffu, !finite) >> (threadIdx.x & 28) & 15u;
+  return !others && wide_rule(n & 0xffffffu, n >> 24, left);
+}
+// Whether two planes leave anything of a piece, and whether that has to be looked at (any of a warp's groups may be wide).  They leave nothing of a value
+// whose leading code is 2^-5 or more (it is 2^-6 * 2^E or more, its last bit 2^-13 * 2^E or more and so no less than the remainder plane's last step, whose
+// scale is 2^(E - 4) at most, half a step of 448's binade being 16 < 448 * 2^-4; and what the leading plane leaves of it is at most 8 such bits), and
+// at most 2^-14 * 2^E, or the value, of a smaller one.
+UQ_DEV bool may_leave(uint2 hi) {   // (a byte with an exponent field of 0 or 1: adding 0x70 to its upper three bits does not reach bit 7)
+  return (((hi.x & 0x70707070u) + 0x70707070u) & ((hi.y & 0x70707070u) + 0x70707070u) & 0x80808080u) != 0x80808080u;
+}
+// A code's bits are a logarithm as well, 8 to the binade with 56 for 1: where a lane's eight codes are 84 on average (2^3.5 * 2^E), and so all 32, at most
+// 10 values are that small, and even they leave the geometric mean too high for the rule: with n of them at 2^-14 * 2^E it is 2^(3.5 + 0.219 n
+// - 14 n / 32) * 2^E, above 1 for every n up to 10, and smaller ones lose no more than themselves.
+UQ_DEV bool may_be_wide(uint2 hi) { return __dp4a(hi.x & 0x7f7f7f7fu, 0x01010101u, __dp4a(hi.y & 0x7f7f7f7fu, 0x01010101u, 0u)) < 8u * 84u; }
+// A code's value, and the code of one value.
+UQ_DEV float e4m3_value(uint32_t code) {
+  float lo, hi;
+  e4m3x2_to_f32(code, lo, hi);
+  return lo;
 }
 
 }  // namespace mx8

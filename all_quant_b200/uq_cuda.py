@@ -590,7 +590,9 @@ def fp4_linear(x, wc, ws, n=None, *, scales=None, out=None, out_dtype=None, work
     is served; the weight is read once per 64 bf16 or 128 8-bit rows).  fp32 sums, rounded once.
 
     x bf16 [..., K], or float8_e4m3fn [..., K] with scales uint8 [..., K/32] (what rms_norm_mx8 and silu_mul_mx8 return);
-    bf16 values are taken exactly, save for what lies under 2^-21 of the largest of their 32 channels.  n: output channels
+    bf16 values are taken exactly, save that of 32 channels the smallest may lose up to 2^-14 of the geometric mean of those that are not zero, and no more
+    than 2^-21 of the largest; where two 8-bit parts would lose more (a channel some thousand times the others) they are taken in four, the call
+    then takes longer (by half for three such channels, many times for one in every 32).  n: output channels
     (default: all rows of the tiles).  out_dtype bf16 (default), fp16 or fp32, or `out` [..., n].  workspace: uint8 scratch of
     fp4_linear_scratch_bytes(rows, K) bytes for bf16 rows (nothing is allocated inside then, out given).  Returns [..., n]."""
     return (_host_module or _host()).fp4_linear(x, wc, ws, n, scales, out, out_dtype, workspace)

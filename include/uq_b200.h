@@ -115,7 +115,8 @@ int uqb_silu_mul_mx8_launch(const void* x, uint8_t* codes, uint8_t* scales, long
  *               scales [ceil(N/128), ceil(K/128), 128, 4]; row n of the weight is token n % 128 of page n / 128, channels
  *               128 h.. are head h.  uqb_append_ex_launch writes it (key = the weight as [N, K/128, 128], slots 0..N-1);
  *               channels behind K and rows behind N have finite scales (the append leaves zero codes there when they are zero).
- *   x, xs       xs NULL: x is bf16 [M, K], taken as two e4m3 planes (exact but for what lies under 2^-21 of a group's largest),
+ *   x, xs       xs NULL: x is bf16 [M, K], taken as two e4m3 planes; of a group of 32 channels the smallest may lose up to 2^-14 of the geometric mean of
+ *               those that are not zero (and at most 2^-21 of the largest); where it were more, four planes are taken (the call then takes longer);
  *               scratch holds uqb_fp4_linear_scratch_bytes(M, K) bytes (none up to 4 rows: may be NULL); else x e4m3 [M, K], xs its scale bytes [M, K/32].
  *   out         [M, N], out_dtype 0 = fp32, 1 = bf16, 2 = fp16.
  * Every wait on the device is bounded; should one run out, outputs of that call are NaN and uqb_last_status says so.

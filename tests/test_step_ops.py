@@ -858,3 +858,88 @@ def test_norm_of_tiny_rows(dtype, H, eps):
     r = 1 / np.sqrt(((2 * x64) ** 2).mean(-1, keepdims=True) + float(np.float32(eps)))
     check_mx8(codes, scales, 2 * x64 * r * w64)
     assert (_f64(s) == 2 * x64).all()
+
+
+def check_wide_range(y, x64, w64, dtype):
+    """Products of bf16 rows whose groups span many binades: tighter than check_linear's `split`, whose bound is the group's largest value alone.
+    What two planes leave out of a value is at most half a step of the second one, 2^-21 of the group's largest, and never more than the value.  It is let go
+    where it is at most 2^-14 of the group's geometric mean (of the values that are not zero, by their bits); else two more planes hold it but for
+    2^-21 of the largest that was left.  A wide group's channels are added in two steps more."""
+    x = np.abs(x64).reshape(len(x64), -1, 32)
+    bits = (x.astype(np.float32).view(np.uint32) >> 16).astype(np.int64)
+    mean = ((bits.sum(2) // np.maximum((bits > 0).sum(2), 1)).astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+    left = np.minimum(x, 2.0 ** -21 * x.max(2, keepdims=True))
+    lost = np.minimum(left, np.maximum(2.0 ** -14 * mean, 2.0 ** -21 * left.max(2))[..., None])
+    A, K = np.abs(x64) @ np.abs(w64).T, x64.shape[1]
+    y64 = x64 @ w64.T
+    tol = (2 * K / 32 + 32) * 2.0 ** -22 * 1.125 * A + torch.finfo(dtype).eps / 2 * np.abs(y64) + lost.reshape(x64.shape) @ np.abs(w64).T
+    assert (np.abs(y.double().cpu().numpy() - y64) <= tol).all()
+
+
+def _wide_rows(M, K, every, ratio, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(M, K, generator=g, device="cuda")
+    x[:, 5::every] *= ratio
+    return x.bfloat16()
+
+
+@gpu
+@pytest.mark.parametrize("every,ratio", [(1 << 20, 1e5), (32, 1e3), (32, 16384.0), (8, 1e5), (4, 1e3), (32, 1e9), (512, 1e30)])
+@pytest.mark.parametrize("M,N,K", [(1, 200, 1024), (3, 130, 2080), (4, 256, 4096), (5, 200, 2080), (8, 128, 4096), (9, 300, 96), (16, 256, 1056), (20, 130, 2048), (33, 257, 1120), (64, 300, 2048),
+                                   (100, 128, 1024), (64, 19100, 416)])
+def test_linear_of_rows_with_large_channels(M, N, K, every, ratio):
+    """A channel far larger than the others of its 32 whose codes in the weight are zero: the others count as they would without it."""
+    g = torch.Generator(device="cuda").manual_seed(N)
+    w = torch.randn(N, K, generator=g, device="cuda") * K ** -0.5
+    w[:, 5::every] = 0
+    wc, ws = uq_cuda.pack_fp4_weight(w)
+    x = _wide_rows(M, K, every, ratio, M)
+    w64 = weight64(wc, ws, N, K)
+    assert (w64[:, 5::every] == 0).all()
+    check_wide_range(uq_cuda.fp4_linear(x, wc, ws, N, out_dtype=torch.float32), _f64(x), w64, torch.float32)
+    check_wide_range(uq_cuda.fp4_linear(x, wc, ws, N), _f64(x), w64, torch.bfloat16)
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(4, 200, 2048), (6, 200, 2048), (16, 256, 1056), (24, 200, 2048), (50, 300, 2048), (64, 19100, 416)])
+def test_wide_rows_leave_their_neighbours_alone_and_repeat(M, N, K):
+    """A row's bits do not depend on whether the rows beside it are of wide range, and are the same every time."""
+    wc, ws = _weight(N, K, 4)
+    x = _rand((M, K), torch.bfloat16, 5)
+    plain = uq_cuda.fp4_linear(x, wc, ws, N, out_dtype=torch.float32)
+    mixed = x.clone()
+    mixed[1::2] = _wide_rows(M, K, 32, 1e5, 6)[1::2]
+    mixed[1, 7] = float("inf")
+    want = uq_cuda.fp4_linear(mixed, wc, ws, N, out_dtype=torch.float32)
+    assert torch.equal(want[::2], plain[::2]) and want[1].isnan().all() and not want[2:].isnan().any()
+    for _ in range(10):
+        assert torch.equal(uq_cuda.fp4_linear(mixed, wc, ws, N, out_dtype=torch.float32)[2:], want[2:])
+    work = torch.full((uq_cuda.fp4_linear_scratch_bytes(M, K),), 255, dtype=torch.uint8, device="cuda")
+    assert torch.equal(uq_cuda.fp4_linear(mixed, wc, ws, N, out_dtype=torch.float32, workspace=work)[2:], want[2:])
+
+
+@gpu
+def test_linear_picks_single_channels_of_any_size():
+    """A weight of one channel per row: y is that channel.  To 2^-7 of itself or what an ordinary group's typical magnitude allows, whatever lies beside it."""
+    K = 256
+    w = torch.zeros(K, K, device="cuda")
+    w[torch.arange(K), torch.arange(K)] = 1
+    wc, ws = uq_cuda.pack_fp4_weight(w)
+    for M in (2, 7, 12, 30, 60):
+        x = (torch.randn(M, K, generator=torch.Generator(device="cuda").manual_seed(M), device="cuda") * torch.tensor([1e-20, 1.0, 1e4, 1e9], device="cuda").repeat(K // 4)).bfloat16()
+        check_wide_range(uq_cuda.fp4_linear(x, wc, ws, out_dtype=torch.float32), _f64(x), weight64(wc, ws, K, K), torch.float32)
+
+
+@gpu
+def test_linear_of_more_steps_than_a_cta_has_marks():
+    """1172 steps of a CTA: a mark stands for two of them."""
+    M, N, K = 5, 128, 1200000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.randn(N, K, generator=g, device="cuda")
+    w[:, 5::50000] = 0
+    wc, ws = uq_cuda.pack_fp4_weight(w)
+    x = torch.randn(M, K, generator=g, device="cuda")
+    x[:, 5::50000] *= 1e6
+    x = x.bfloat16()
+    w64 = weight64(wc, ws, N, K)
+    check_wide_range(uq_cuda.fp4_linear(x, wc, ws, out_dtype=torch.float32), _f64(x), w64, torch.float32)
