@@ -60,6 +60,11 @@ Tensor rows(const Tensor& t) {
   Tensor c = t.contiguous();
   return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) ? c.clone() : c;
 }
+// Do two contiguous tensors share memory?
+bool overlap(const Tensor& a, const Tensor& b) {
+  const char *p = static_cast<const char*>(a.data_ptr()), *q = static_cast<const char*>(b.data_ptr());
+  return p < q + b.nbytes() && q < p + a.nbytes();
+}
 int dtype_code(at::ScalarType t) { return t == at::kFloat ? 0 : (t == at::kBFloat16 ? 1 : (t == at::kHalf ? 2 : -1)); }
 void done(int err, const char* what) {
   REFUSE(err == 1, what, " failed: cudaErrorInvalidValue (shape not served / bad argument)");
@@ -241,6 +246,9 @@ PyObject* fp4_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   shape.back() = n;
   if (!out) out = fresh(shape, od, place);
   else REFUSE(out->scalar_type() != od || out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous(), "out must be contiguous bf16, fp16 or fp32 [..., n]");
+  // (the kernels' CTAs read x until the last one is done, while others write their channels of out)
+  if (overlap(*out, x)) x = x.clone();
+  if (scales && overlap(*out, *scales)) scales = scales->clone();
   const c10::cuda::CUDAGuard on(place.device);
   done(linear_fn(x.data_ptr(), static_cast<uint8_t*>(ptr(scales)), static_cast<uint8_t*>(wc.data_ptr()), static_cast<uint8_t*>(ws.data_ptr()), out->data_ptr(),
                  scales ? nullptr : ptr(work), M, (int)n, (int)K, dtype_code(od), stream_of(place)),

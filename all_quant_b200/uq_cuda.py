@@ -594,7 +594,8 @@ def fp4_linear(x, wc, ws, n=None, *, scales=None, out=None, out_dtype=None, work
     than 2^-21 of the largest; where two 8-bit parts would lose more (a channel some thousand times the others) they are taken in four, the call
     then takes longer (by half for three such channels, many times for one in every 32).  n: output channels
     (default: all rows of the tiles).  out_dtype bf16 (default), fp16 or fp32, or `out` [..., n].  workspace: uint8 scratch of
-    fp4_linear_scratch_bytes(rows, K) bytes for bf16 rows (nothing is allocated inside then, out given).  Returns [..., n]."""
+    fp4_linear_scratch_bytes(rows, K) bytes for bf16 rows (nothing is allocated inside then, out given, unless out is x's own memory: x is
+    copied first).  Returns [..., n]."""
     return (_host_module or _host()).fp4_linear(x, wc, ws, n, scales, out, out_dtype, workspace)
 
 

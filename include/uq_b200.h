@@ -118,7 +118,7 @@ int uqb_silu_mul_mx8_launch(const void* x, uint8_t* codes, uint8_t* scales, long
  *   x, xs       xs NULL: x is bf16 [M, K], taken as two e4m3 planes; of a group of 32 channels the smallest may lose up to 2^-14 of the geometric mean of
  *               those that are not zero (and at most 2^-21 of the largest); where it were more, four planes are taken (the call then takes longer);
  *               scratch holds uqb_fp4_linear_scratch_bytes(M, K) bytes (none up to 4 rows: may be NULL); else x e4m3 [M, K], xs its scale bytes [M, K/32].
- *   out         [M, N], out_dtype 0 = fp32, 1 = bf16, 2 = fp16.
+ *   out         [M, N], out_dtype 0 = fp32, 1 = bf16, 2 = fp16; shares no memory with the others.
  * Every wait on the device is bounded; should one run out, outputs of that call are NaN and uqb_last_status says so.
  * K a multiple of 32, wc 32-byte aligned, x / ws / scratch 16, xs 4, out as four of its values (as one where N is no multiple of 4).  A row of x that holds NaN or infinity (bf16), or a
  * NaN code, gives NaN in its outputs; other rows are not touched by it. */

@@ -943,3 +943,41 @@ def test_linear_of_more_steps_than_a_cta_has_marks():
     x = x.bfloat16()
     w64 = weight64(wc, ws, N, K)
     check_wide_range(uq_cuda.fp4_linear(x, wc, ws, out_dtype=torch.float32), _f64(x), w64, torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 4, 9, 40])
+def test_linear_into_its_own_input(M):
+    """out in x's memory: every CTA reads all of x, and none may find another's outputs there."""
+    K = 4096
+    wc, ws = _weight(K, K, 7)
+    x = _wide_rows(M, K, 500, 1e5, M)
+    want = uq_cuda.fp4_linear(x, wc, ws)
+    for _ in range(5):
+        mine = x.clone()
+        assert uq_cuda.fp4_linear(mine, wc, ws, out=mine) is mine and torch.equal(mine, want)
+        both = torch.cat([x.view(-1), x.view(-1)])   # one that begins in the middle of x
+        assert torch.equal(uq_cuda.fp4_linear(both[:M * K].view(M, K), wc, ws, out=both[M * K // 2:M * K // 2 + M * K].view(M, K)), want)
+    codes, scales, _ = uq_cuda.rms_norm_mx8(x)
+    want = uq_cuda.fp4_linear(codes, wc, ws, scales=scales)
+    buf = torch.empty(M, K, dtype=torch.bfloat16, device="cuda")
+    mine = buf.view(torch.uint8).view(-1)[:M * K].view(M, K).view(torch.float8_e4m3fn)
+    mine.copy_(codes)
+    assert torch.equal(uq_cuda.fp4_linear(mine, wc, ws, scales=scales, out=buf), want)
+    s = buf.view(torch.uint8).view(-1)[M * K:M * K + M * K // 32].view(M, K // 32)
+    s.copy_(scales)
+    assert torch.equal(uq_cuda.fp4_linear(codes, wc, ws, scales=s, out=buf), want)
+
+
+@gpu
+def test_linear_into_its_own_input_with_more_tiles_than_the_device_holds():
+    """The same where some CTAs start when others have long written theirs."""
+    M, K = 2, 40960
+    g = torch.Generator(device="cuda").manual_seed(1)
+    wc = torch.randint(0, 256, (K // 128, K // 128, 128, 64), generator=g, device="cuda", dtype=torch.uint8)
+    ws = torch.full((K // 128, K // 128, 128, 4), 120, dtype=torch.uint8, device="cuda")
+    x = _rand((M, K), torch.bfloat16, 3)
+    want = uq_cuda.fp4_linear(x, wc, ws)
+    for _ in range(3):
+        mine = x.clone()
+        assert torch.equal(uq_cuda.fp4_linear(mine, wc, ws, out=mine), want)
