@@ -65,6 +65,10 @@ bool overlap(const Tensor& a, const Tensor& b) {
   const char *p = static_cast<const char*>(a.data_ptr()), *q = static_cast<const char*>(b.data_ptr());
   return p < q + b.nbytes() && q < p + a.nbytes();
 }
+// An input that shares memory with an output is copied, unless they are the same elements (`in_place`: every thread reads its own before it writes them).
+void apart(Tensor& in, const optional<Tensor>& out, bool in_place = false) {
+  if (out && overlap(in, *out) && !(in_place && in.data_ptr() == out->data_ptr())) in = in.clone();
+}
 int dtype_code(at::ScalarType t) { return t == at::kFloat ? 0 : (t == at::kBFloat16 ? 1 : (t == at::kHalf ? 2 : -1)); }
 void done(int err, const char* what) {
   REFUSE(err == 1, what, " failed: cudaErrorInvalidValue (shape not served / bad argument)");
@@ -167,6 +171,11 @@ PyObject* rms_norm_mx8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!sum) sum = fresh(x.sizes(), dt, place);
   }
   mx8_out(x, H, place, codes, scales);
+  for (const auto* t : {&codes, &scales, &sum}) {
+    apart(x, *t, t == &sum);
+    if (r) apart(*r, *t, t == &sum);
+    if (w) apart(*w, *t);
+  }
   const c10::cuda::CUDAGuard on(place.device);
   done(norm_fn(x.data_ptr(), ptr(r), ptr(w), ptr(sum), static_cast<uint8_t*>(codes->data_ptr()), static_cast<uint8_t*>(scales->data_ptr()), x.numel() / H, (int)H, dtype_code(dt),
                (float)eps, stream_of(place)),
@@ -190,6 +199,8 @@ PyObject* silu_mul_mx8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   REFUSE(F2 < 64 || F2 % 64 || F2 > (1 << 21), "silu_mul_mx8: twice a multiple of 32 channels, up to 2^21 of them");
   x = rows(x);
   mx8_out(x, F2 / 2, place, codes, scales);
+  apart(x, codes);
+  apart(x, scales);
   const c10::cuda::CUDAGuard on(place.device);
   done(silu_fn(x.data_ptr(), static_cast<uint8_t*>(codes->data_ptr()), static_cast<uint8_t*>(scales->data_ptr()), x.numel() / F2, (int)(F2 / 2), dtype_code(x.scalar_type()),
                stream_of(place)),
@@ -247,8 +258,8 @@ PyObject* fp4_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (!out) out = fresh(shape, od, place);
   else REFUSE(out->scalar_type() != od || out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous(), "out must be contiguous bf16, fp16 or fp32 [..., n]");
   // (the kernels' CTAs read x until the last one is done, while others write their channels of out)
-  if (overlap(*out, x)) x = x.clone();
-  if (scales && overlap(*out, *scales)) scales = scales->clone();
+  apart(x, out);
+  if (scales) apart(*scales, out);
   const c10::cuda::CUDAGuard on(place.device);
   done(linear_fn(x.data_ptr(), static_cast<uint8_t*>(ptr(scales)), static_cast<uint8_t*>(wc.data_ptr()), static_cast<uint8_t*>(ws.data_ptr()), out->data_ptr(),
                  scales ? nullptr : ptr(work), M, (int)n, (int)K, dtype_code(od), stream_of(place)),

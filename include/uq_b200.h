@@ -102,7 +102,7 @@ int uqb_plan_step_launch(const int32_t* seq_lens, const int32_t* starts, int K, 
 /* 8-bit rows: e4m3 codes [rows, H] and one scale byte per 32 channels [rows, H/32], value = code * 2^(byte - 127), byte the
  * least with which nothing is clipped (0 for a group of zeros).  Values that are not finite get the NaN code.
  * dtype 0 = fp32, 1 = bf16, 2 = fp16 (of x, residual, weight and sum); H (F) a multiple of 32; codes 8-byte aligned, the
- * others 16.
+ * others 16.  Outputs share no memory with inputs, but for sum as said below.
  *   rms_norm:  s = x + residual (NULL: x), codes of s / sqrt(mean(s^2) + eps) * weight (NULL: ones), in fp32 throughout; sum
  *              [rows, H] gets s rounded to dtype (NULL exactly when residual is; may be x or residual itself).  H <= 32768, eps >= 2^-126.
  *   silu_mul:  x [rows, 2 F] = gates, then factors: codes of g / (1 + exp(-g)) * u. */

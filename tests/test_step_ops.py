@@ -981,3 +981,29 @@ def test_linear_into_its_own_input_with_more_tiles_than_the_device_holds():
     for _ in range(3):
         mine = x.clone()
         assert torch.equal(uq_cuda.fp4_linear(mine, wc, ws, out=mine), want)
+
+
+@gpu
+def test_row_operators_into_their_own_inputs():
+    """Codes, scales or the sum in memory of an input, not the same elements: the input is read as it was."""
+    R, H = 3000, 512
+    x, r, w = _rand((R, H), torch.bfloat16, 1), _rand((R, H), torch.bfloat16, 2), _rand((H,), torch.bfloat16, 3)
+    same = lambda a, b: all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(a, b))
+    want = uq_cuda.rms_norm_mx8(x, w, r)
+    for _ in range(3):
+        for first in (0, 1):   # which input shares its memory
+            args = [x, r]
+            buf = torch.cat([args[first].view(-1), torch.zeros(8 * H, dtype=torch.bfloat16, device="cuda")])
+            args[first] = buf[:R * H].view(R, H)
+            assert same(uq_cuda.rms_norm_mx8(args[0], w, args[1], sum_out=buf[7 * H:(R + 7) * H].view(R, H)), want)
+        mine = x.clone()
+        codes = mine.view(torch.uint8).view(-1)[R * H:].view(R, H).view(torch.float8_e4m3fn)   # the rows' second half
+        assert same(uq_cuda.rms_norm_mx8(mine, w, r, codes=codes), want)
+        mine = x.clone()
+        scales = mine.view(torch.uint8).view(-1)[-R * H // 32:].view(R, H // 32)
+        assert same(uq_cuda.rms_norm_mx8(mine, w, r, scales=scales), want)
+        mine = x.clone()
+        codes = mine.view(torch.uint8).view(-1)[:R * H // 2].view(R, H // 2).view(torch.float8_e4m3fn)
+        assert same(uq_cuda.silu_mul_mx8(mine, codes=codes), uq_cuda.silu_mul_mx8(x))
+    weight = torch.cat([w, torch.zeros(R * H // 32, dtype=torch.bfloat16, device="cuda")])
+    assert same(uq_cuda.rms_norm_mx8(x, weight[:H], r, scales=weight.view(torch.uint8)[:R * H // 32].view(R, H // 32)), want)
