@@ -164,18 +164,20 @@ PyObject* rms_norm_mx8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   REFUSE(sum && !r, "sum_out goes with a residual");
   REFUSE(sum && (sum->scalar_type() != dt || sum->sizes() != x.sizes() || !sum->is_contiguous() || (reinterpret_cast<uintptr_t>(sum->data_ptr()) & 15)),
          "sum_out must be contiguous, 16-byte aligned, of x's shape and type");
+  const bool given_sum = sum.has_value();
   x = rows(x);
   if (w) w = rows(*w);
   if (r) {
     r = rows(*r);
     if (!sum) sum = fresh(x.sizes(), dt, place);
   }
+  if (codes || scales || given_sum)   // (new memory is nobody else's)
+    for (const auto* t : {&codes, &scales, &sum}) {
+      apart(x, *t, t == &sum);
+      if (r) apart(*r, *t, t == &sum);
+      if (w) apart(*w, *t);
+    }
   mx8_out(x, H, place, codes, scales);
-  for (const auto* t : {&codes, &scales, &sum}) {
-    apart(x, *t, t == &sum);
-    if (r) apart(*r, *t, t == &sum);
-    if (w) apart(*w, *t);
-  }
   const c10::cuda::CUDAGuard on(place.device);
   done(norm_fn(x.data_ptr(), ptr(r), ptr(w), ptr(sum), static_cast<uint8_t*>(codes->data_ptr()), static_cast<uint8_t*>(scales->data_ptr()), x.numel() / H, (int)H, dtype_code(dt),
                (float)eps, stream_of(place)),
@@ -198,9 +200,9 @@ PyObject* silu_mul_mx8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t F2 = x.dim() ? x.size(-1) : 0;
   REFUSE(F2 < 64 || F2 % 64 || F2 > (1 << 21), "silu_mul_mx8: twice a multiple of 32 channels, up to 2^21 of them");
   x = rows(x);
-  mx8_out(x, F2 / 2, place, codes, scales);
   apart(x, codes);
   apart(x, scales);
+  mx8_out(x, F2 / 2, place, codes, scales);
   const c10::cuda::CUDAGuard on(place.device);
   done(silu_fn(x.data_ptr(), static_cast<uint8_t*>(codes->data_ptr()), static_cast<uint8_t*>(scales->data_ptr()), x.numel() / F2, (int)(F2 / 2), dtype_code(x.scalar_type()),
                stream_of(place)),
@@ -255,11 +257,14 @@ PyObject* fp4_linear(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     REFUSE(work && (work->scalar_type() != at::kByte || work->numel() < need || !work->is_contiguous()), "scratch too small");
   }
   shape.back() = n;
-  if (!out) out = fresh(shape, od, place);
+  const bool given = out.has_value();
+  if (!given) out = fresh(shape, od, place);
   else REFUSE(out->scalar_type() != od || out->sizes() != at::IntArrayRef(shape) || !out->is_contiguous(), "out must be contiguous bf16, fp16 or fp32 [..., n]");
   // (the kernels' CTAs read x until the last one is done, while others write their channels of out)
-  apart(x, out);
-  if (scales) apart(*scales, out);
+  if (given) {
+    apart(x, out);
+    if (scales) apart(*scales, out);
+  }
   const c10::cuda::CUDAGuard on(place.device);
   done(linear_fn(x.data_ptr(), static_cast<uint8_t*>(ptr(scales)), static_cast<uint8_t*>(wc.data_ptr()), static_cast<uint8_t*>(ws.data_ptr()), out->data_ptr(),
                  scales ? nullptr : ptr(work), M, (int)n, (int)K, dtype_code(od), stream_of(place)),
