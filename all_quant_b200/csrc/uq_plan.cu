@@ -7,8 +7,9 @@
 //   table[b, held_b + j] = free[off_b + j], j < need_b
 //   slot[t] = table[b, p / PAGE] * PAGE + p % PAGE, with p = len_b - n_b + (t - start_b) for token t of request b
 //
-// Bound by latency: lengths -> prefix sums -> bisection -> table -> slot, one after the other, behind a launch (2.9 us from a graph for 2
-// requests, 4.7 for 300 with 77 K new tokens, 6.6 for 64 prompts of 295 K tokens; their bytes would take 0.3 at the most).
+// Bound by latency: lengths -> prefix sums -> bisection -> table -> slot, one after the other, behind a launch (3.0 us from a graph for 2
+// requests, 4.6 for 300 with 73 121 new tokens, 6.6 for 64 prompts of 257 430 tokens; their bytes would take 0.3 at the most).  The last one's 503 blocks
+// are more than the device holds at once (three per SM): those that start late go through the chain again.
 // One launch, nothing kept between blocks: every block works the two prefix sums (pages, tokens) out for itself in shared memory
 // (a few KB of lengths out of L2), then takes its share of the tokens and of the pages handed out.  A token finds its request by
 // bisection of the starts; a page that this step hands out is read from the free list, never from the table, so that no block
@@ -20,7 +21,7 @@
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kTokensPerBlock = kThreads;       // tokens a block is launched for (four times as many, with 64-bit divisions: 8.3 us for 300 requests, 4.8 so)
+constexpr int kTokensPerBlock = kThreads;       // tokens a block is launched for (one / two / four per thread: 300 requests 4.6 / 5.5 / 7.6 us, 64 prompts 6.6 / 6.7 / 6.3)
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRequests = 16384;             // two prefix sums and a position of 4 bytes each in shared memory
 

@@ -4,7 +4,7 @@
 //
 //   quantiser   E = the least integer with amax <= 448 * 2^E (the cache's "ceil" rule with e4m3's largest value: nothing is
 //               clipped), byte = E + 127, code = e4m3(y * 2^-E) to nearest, ties to even; a group of zeros has byte 0.
-//               A value that is not finite has the NaN code (e4m3 has no infinity).
+//               A y that is not finite has the NaN code (e4m3 has no infinity).
 //   norm        s = x + r, y = s * rsqrt(mean(s^2) + eps) * w.  s is kept in fp32 for the norm; the sum that is handed on
 //               (the next residual) is s rounded once to the input's type, as any other addition in that type would leave it.
 //   gate        y = g / (1 + exp(-g)) * u
@@ -15,7 +15,8 @@
 // A lane owns pieces of 8 channels (one 16-byte load of a 16-bit type), a group of 32 is four lanes, whose maximum takes two shuffles;
 // a piece leaves as one 8-byte store.  Memory should bound all three, and does where a value brings 7 bytes (norm of 16384 x 8192 bf16 with a
 // residual: 138 us from a graph, 6.8 TB/s); with 3 and 5 bytes the issue slots run out first (norm of 8191 x 4096 fp16 23 us, 4.4 TB/s, 16
-// instructions per value; gate of 5001 x 11040 bf16 54 us, 5.1 TB/s, 24), hence the paired arithmetic.
+// instructions per value; gate of 5001 x 11040 bf16 52 to 58 us on different boxes, 4.8 to 5.3 TB/s, 24), hence the paired arithmetic.  fp32: gate of 4096 x 8192 47 us,
+// 6.5 TB/s; norm of 8192 x 4096 with a residual 79 us, 5.6 TB/s (four pieces of fp32 do not fit 64 registers: 72 bytes of stack).
 #include <atomic>
 #include <climits>
 

@@ -551,7 +551,7 @@ def rms_norm_mx8(x, weight=None, residual=None, *, eps=1e-6, codes=None, scales=
     x [..., H] fp32, bf16 or fp16, H a multiple of 32 up to 32768; residual of x's shape and weight [H] of x's dtype (None:
     nothing added / ones).  Returns (codes float8_e4m3fn [..., H], scales uint8 [..., H/32], s rounded to x's dtype - the next
     residual; None without one).  sum_out may be x or residual itself (in place).  The norm is taken of s in fp32, before it is
-    rounded.  Rows holding NaN or infinity give NaN codes."""
+    rounded.  A row that holds a NaN gives NaN codes; one that holds an infinity NaN there and zeros elsewhere, as the formula has it."""
     return (_host_module or _host()).rms_norm_mx8(x, weight, residual, eps, codes, scales, sum_out)
 
 

@@ -100,7 +100,8 @@ int uqb_plan_step_launch(const int32_t* seq_lens, const int32_t* starts, int K, 
                          long long n_free, int64_t* slots, int32_t* taken, int B, long long T, int PAGE, int max_pages, void* stream);
 
 /* 8-bit rows: e4m3 codes [rows, H] and one scale byte per 32 channels [rows, H/32], value = code * 2^(byte - 127), byte the
- * least with which nothing is clipped (0 for a group of zeros).  Values that are not finite get the NaN code.
+ * least with which nothing is clipped (0 for a group of zeros).  Values (of the result) that are not finite get the NaN code: of a row
+ * with a NaN all, of a norm's row with an infinity that one (the others are zeros).
  * dtype 0 = fp32, 1 = bf16, 2 = fp16 (of x, residual, weight and sum); H (F) a multiple of 32; codes 8-byte aligned, the
  * others 16.  Outputs share no memory with inputs, but for sum as said below.
  *   rms_norm:  s = x + residual (NULL: x), codes of s / sqrt(mean(s^2) + eps) * weight (NULL: ones), in fp32 throughout; sum

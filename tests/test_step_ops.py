@@ -1007,3 +1007,33 @@ def test_row_operators_into_their_own_inputs():
         assert same(uq_cuda.silu_mul_mx8(mine, codes=codes), uq_cuda.silu_mul_mx8(x))
     weight = torch.cat([w, torch.zeros(R * H // 32, dtype=torch.bfloat16, device="cuda")])
     assert same(uq_cuda.rms_norm_mx8(x, weight[:H], r, scales=weight.view(torch.uint8)[:R * H // 32].view(R, H // 32)), want)
+
+
+def test_no_wide_group_is_overlooked():
+    """The products' rule for groups of wide range (what two planes leave out of a value is more than 2^-14 of the geometric mean) is only asked where a lane's
+    eight leading codes are, as whole numbers, under 84 on average: in numpy, over groups made to come close - a few values at, around and far below
+    the border where two planes begin to lose bits, zeros among them - no group that the rule calls wide is passed over."""
+    rng = np.random.default_rng(1)
+    bf16 = lambda x: ((np.asarray(x, np.float32).view(np.uint32) + 0x8000) & np.uint32(0xffff0000)).view(np.float32).astype(np.float64)
+    wide_groups = 0
+    for _ in range(20):
+        N = 10000
+        v, low = rng.standard_normal((N, 32)), np.arange(32) < rng.integers(0, 32, (N, 1))
+        kind, top = rng.integers(0, 6, (N, 1)), np.abs(v).max(1, keepdims=True)
+        size = 2.0 ** rng.uniform(-40, 2, (N, 1))
+        v = np.select([(kind == 0) & low, (kind == 1) & low, (kind == 2) & low, (kind == 3) & low, kind == 3, (kind == 4) & low, kind == 5],
+                      [v * size, v * 2.0 ** rng.uniform(-30, 0, (N, 32)), top * 2.0 ** -14 * rng.uniform(0.3, 1, (N, 32)), np.sign(v) * size * rng.uniform(0.5, 1, (N, 32)),
+                       448 * rng.uniform(0.5, 1, (N, 32)), np.zeros_like(v), v ** 5], v)
+        x = bf16(v)
+        E = exponent(np.abs(x).max(1))[:, None]
+        hi = e4m3(np.ldexp(x, -E))
+        rest = x - np.ldexp(hi, E)
+        E2 = exponent(np.abs(rest).max(1))[:, None]
+        left = np.abs(rest - np.ldexp(e4m3(np.ldexp(rest, -E2)), E2)).max(1)
+        bits = (np.abs(x).astype(np.float32).view(np.uint32) >> 16).astype(np.int64)
+        mean = ((bits.sum(1) // np.maximum((bits > 0).sum(1), 1)).astype(np.uint32) << 16).view(np.float32)
+        codes = torch.from_numpy(np.abs(hi)).to(torch.float8_e4m3fn).view(torch.uint8).numpy().astype(np.int64).reshape(N, 4, 8).sum(2)
+        wide = left > 2.0 ** -14 * mean
+        wide_groups += wide.sum()
+        assert ((codes < 8 * 84).any(1) | ~wide).all()
+    assert wide_groups > 20000
