@@ -215,14 +215,35 @@ UQ_DEV void extra_rows(const LinearParams& p, int m0, int rows, int k, int warp,
     *reinterpret_cast<uint4*>(t1 + at) = *reinterpret_cast<uint4*>(t1 + ROWS * 128 + at) = make_uint4(0, 0, 0, 0);
   }
   auto scales_of = [](int r) { return (r & 31) * 16 + (r >> 5) * 4; };
-  uint32_t groups = 0;   // of row r0 + lane
+  uint32_t groups = 0;   // of row r0 + lane, the wide ones
+  if constexpr (kDirect) {   // as they were found before: eight channels per lane, two rows at a time
+    uint32_t mine = 0;
+#pragma unroll 1
+    for (int j = 0; j < kDirectRows / 2; j++) {
+      const int r = 2 * j + (lane >> 4), c = 128 * k + 8 * (lane & 15);
+      mx8::Raw<__nv_bfloat16> x;
+      x.a = make_uint4(0, 0, 0, 0);
+      if (r < rows && c < p.K) x.load(p.x16 + (long long)(m0 + r) * p.K + c);
+      float v[8];
+      x.get(v);
+      uint2 hi, lo;
+      uint32_t hi_byte, lo_byte;
+      mx8::split_piece(v, hi, lo, hi_byte, lo_byte);
+      const uint32_t wide = __ballot_sync(0xffffffffu, wide_group_far(x.a, hi, lo, hi_byte, lo_byte));
+      if (lane >> 1 == j) mine = wide >> 16 * (lane & 1);
+    }
+    groups = (mine & 1u) | (mine >> 3 & 2u) | (mine >> 6 & 4u) | (mine >> 9 & 8u);   // (four lanes a group)
+  }
   if (lane < n) {
     const int r = r0 + lane;
     *reinterpret_cast<uint32_t*>(s0 + scales_of(r)) = *reinterpret_cast<uint32_t*>(s0 + scales_of(ROWS + r)) = 0x01010101u;
     *reinterpret_cast<uint32_t*>(s1 + scales_of(r)) = *reinterpret_cast<uint32_t*>(s1 + scales_of(ROWS + r)) = 0x01010101u;
-    if (r < rows)
+    if (!kDirect && r < rows) {
+      const uint8_t* bytes = p.xs + (long long)(2 * m0 + r) * (p.K / 32) + 4 * k;   // (m0: a multiple of ROWS)
+      const uint32_t four = p.words ? *reinterpret_cast<const uint32_t*>(bytes) : 0u;
       for (int g = 0; g < 4 && 4 * k + g < p.K / 32; g++)
-        if (kDirect || p.xs[(long long)(2 * m0 + r) * (p.K / 32) + 4 * k + g] == mx8::kWideByte) groups |= 1u << g;   // (m0: a multiple of ROWS)
+        if ((p.words ? four >> 8 * g & 0xffu : (uint32_t)bytes[g]) == mx8::kWideByte) groups |= 1u << g;
+    }
   }
   __syncwarp();
   int r = -1;
@@ -242,26 +263,21 @@ UQ_DEV void extra_rows(const LinearParams& p, int m0, int rows, int k, int warp,
 #pragma unroll 1
   while (g >= 0) {
     const int row = r0 + r, c = 32 * g + lane;
-    const uint32_t bits = x & 0x7fffu;
     float v = __uint_as_float(x << 16);
     uint8_t* at0 = t0 + row * 128 + (((c >> 4) ^ (row & 7)) << 4) + (c & 15);
     const int to1 = (int)(t1 - t0), sf = scales_of(row) + g, sf2 = scales_of(ROWS + row) + g;
     g = next();
     if (g >= 0) x = load(g);
-    if (kDirect && __any_sync(0xffffffffu, bits >= 0x7f80u)) continue;
     uint32_t codes = 0;   // four planes' and their bytes
     uint32_t bytes = 0;
-    bool wide = true;
 #pragma unroll 1
     for (int i = 0; i < 32; i += 8) {
       const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v))));
-      if (kDirect && i == 16) wide = mx8::wide_rule(__reduce_add_sync(0xffffffffu, bits), __popc(__ballot_sync(0xffffffffu, bits != 0)), amax);
       const uint32_t byte = max(mx8::scale_byte(amax), 1u), code = mx8::e4m3x2(__fmul_rn(v, mx8::inverse_scale(byte)), 0.f) & 0xffu;
       v = fmaf(mx8::e4m3_value(code), -uq_scale_f32(byte), v);
       codes |= code << i;
       bytes |= byte << i;
     }
-    if (!wide) continue;
     at0[0] = (uint8_t)codes;
     at0[ROWS * 128] = (uint8_t)(codes >> 8);
     at0[to1] = (uint8_t)(codes >> 16);

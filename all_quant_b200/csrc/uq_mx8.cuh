@@ -140,16 +140,14 @@ UQ_DEV void split_piece(float* v, uint2& hi, uint2& lo, uint32_t& hi_byte, uint3
   take_out(v, hi, hi_byte);
   plane_of(v, lo, lo_byte);
 }
+
 // ---- groups of wide range ---------------------------------------------------------------------------------------------
 // What two planes leave out of bf16 values lies under 2^-21 of the group's largest, in values below 2^-13 of it.  Where that is an ordinary group's smallest
 // value it is nothing beside the others.  In a group of wide range - a few large channels, whose codes in the weight may be zero - it is not: the group is
 // "wide" where a value loses more than 2^-14 of the group's typical magnitude, the geometric mean of the values that are not zero (a bf16's bits, read
-// as a whole number, are its logarithm but for the mantissa's curve; no large channel moves that mean far).  All of it is whole numbers and maxima: any
-// order of the lanes gives the same answer.  (Normal or Laplace distributed values, or products of two such: not one group of 131 072.  32 values of which
-// 1, 4 or 8 are 1000 times the others: 17 to 29 %, 16 384 times: 86 to 99.7 %.)
+// as a whole number, are its logarithm but for the mantissa's curve; no large channel moves that mean far).  (Normal or Laplace distributed values, or
+// products of two such: not one group of 131 072.  32 values of which 1, 4 or 8 are 1000 times the others: 17 to 29 %, 16 384 times: 86 to 99.7 %.)
 constexpr uint32_t kWideByte = 0;   // in place of such a group's scales, with codes of zero
-UQ_DEV bool wide_rule(uint32_t sum, uint32_t count, float left) { return left > 6.103515625e-05f * __uint_as_float(sum / max(count, 1u) << 16); }
-
 // Whether a lane's group is wide: its piece with its codes and bytes (not for a group with NaN or infinity, whose own codes say it).
 UQ_DEV bool wide_group(uint4 raw, uint2 hi, uint2 lo, uint32_t hi_byte, uint32_t lo_byte) {
   Raw<__nv_bfloat16> x;
@@ -171,7 +169,7 @@ UQ_DEV bool wide_group(uint4 raw, uint2 hi, uint2 lo, uint32_t hi_byte, uint32_t
   n += __shfl_xor_sync(0xffffffffu, n, 1);
   n += __shfl_xor_sync(0xffffffffu, n, 2);
   const uint32_t others = __ballot_sync(0xffffffffu, !finite) >> (threadIdx.x & 28) & 15u;
-  return !others && wide_rule(n & 0xffffffu, n >> 24, left);
+  return !others && left > 6.103515625e-05f * __uint_as_float((n & 0xffffffu) / max(n >> 24, 1u) << 16);   // 2^-14
 }
 // Whether two planes leave anything of a piece, and whether that has to be looked at (any of a warp's groups may be wide).  They leave nothing of a value
 // whose leading code is 2^-5 or more (it is 2^-6 * 2^E or more, its last bit 2^-13 * 2^E or more and so no less than the remainder plane's last step, whose
