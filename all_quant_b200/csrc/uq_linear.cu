@@ -295,6 +295,7 @@ UQ_DEV void extra_rows(const LinearParams& p, int m0, int rows, int k, int warp,
 template <typename C, int kScaleWarps, bool kDirect>
 __device__ __noinline__ bool bring_extra(const LinearParams& p, const CUtensorMap& map_w, uint32_t sm, uint8_t* smem, int nk, int k0, int tile_n, int m0, int rows) {
   constexpr int kGroups = 4 / kScaleWarps;
+  static_assert(C::kStages >= 3, "a pair of steps, and whoever waits for a stage has seen the turn before the last one's end");
   const int warp = threadIdx.x >> 5;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::oAbort);
   bool ok = true;
